@@ -71,11 +71,14 @@ typedef uint64_t sdq_weight_t;
                                 * turns into a relative error of the same size on every weight; see the
                                 * measured figures beside SDQ_SDPA_V_FP16 in the description of sdq_sdpa */
 
+#define SDQ_CAUSAL 0x200u    /* sdq_kv_attention: a row sees the keys up to its own position only */
+
 /* source element types of sdq_quantize_rows (the packer's SRC table,
  * tools/quantize/pack_sdcpp.py:26-35) */
 #define SDQ_F32 0
 #define SDQ_BF16 1
 #define SDQ_F16 2
+#define SDQ_I8 3 /* rows of sdq_w4_matmul that are already quantized */
 
 /* rounding recipe of sdq_quantize_rows */
 #define SDQ_MODE_PACKER 0  /* quant_rows, tools/quantize/pack_sdcpp.py:45-51 */
@@ -305,6 +308,104 @@ SDQ_API int sdq_fmatmul(sdq_weight_t w, const float* A, int64_t M, float* out,
 SDQ_API int sdq_sdpa(const float* q_dev, const float* k_dev, const float* v_dev, int64_t Lq,
                      int64_t Lk, int64_t C, int heads, float* out_dev, uint32_t flags,
                      void* stream);
+
+/* ---- few-bit inference beside the int8 linears ----
+ * The entry points of this section serve transformers that keep their weights in 4 bits and their
+ * keys and values in 8.  They take device pointers only, need nothing beyond the natural alignment
+ * of an element unless they say so (16-byte aligned rows are faster), use no scratch -- calls and
+ * captured graphs on different streams share nothing -- and two runs give the same bits.  `flags`
+ * may carry SDQ_SYNC and what the entry point names; anything else is refused.  Types are SDQ_F32,
+ * SDQ_BF16 and SDQ_F16.  A row stride (ld...) is in elements; 0 stands for rows without a gap.  The
+ * buffers of a call must not overlap except where it says so. */
+
+/* RMS norm with the residual's addition in front and the activation quantization of the int8
+ * linears behind it, in one kernel:
+ *   s = X + residual, rounded to `dtype` and written to sum_out (s = X when residual is NULL);
+ *   h = s / sqrt(mean(s^2) + eps) * weight   (weight fp32 [K], NULL: no weight);
+ *   a_scale = max|h| * (1/127) of the row, 1 where that is below 2^-126;
+ *   aq = h * (1 / a_scale) rounded to nearest even within [-127, 127].
+ * That is sdq_quantize_activations of h but for the last bit of a scale (it divides by 127).
+ * X, residual and sum_out are [M,K] of `dtype`; sum_out may be X or residual itself (then with its
+ * stride) and is given exactly when residual is.  aq (int8 [M,K]) and a_scale (fp32 [M]) go together
+ * and feed sdq_qgemm_prequantized or sdq_w4_matmul; h_out ([M,K] of `dtype`, h rounded once) may be
+ * asked for beside them or, with both NULL, alone (a norm of queries and keys).  The mean and the
+ * root are taken in 64 bits and h in fp32, (s * r) * weight with two roundings, so the bytes do not
+ * depend on the order of the sums.  Replaces sd::rmsnorm in front of a linear
+ * (src/core/tensor.h, src/core/tensor.cpp).  Rows up to 16384 fp32 or 32768 16-bit elements, a
+ * multiple of 16 bytes long and 16-byte aligned, are read once. */
+SDQ_API int sdq_rmsnorm_quantize(const void* X_dev, int dtype, int64_t ldx, const void* residual_dev, int64_t ldr,
+                                 int64_t M, int64_t K, const float* weight_dev, float eps, void* sum_out_dev,
+                                 int64_t lds, int8_t* aq_dev, float* a_scale_dev, void* h_out_dev, uint32_t flags,
+                                 void* stream);
+
+/* 4-bit weights: w[n,k] = q[n,k] * scale[n, k / group], q in [-8, 7], group 32, 64 or 128 columns (the
+ * last one of a row may be shorter).  Packed form: [N, ceil(K/2)] bytes, column 2j in the low and
+ * 2j + 1 in the high nibble of byte j, each nibble q + 8; scales [N, ceil(K/group)] in scale_dtype.
+ * sdq_w4_quantize makes it from [N,K] of src_dtype: scale = max|w| / 7 of the group rounded to
+ * scale_dtype (at most its largest finite number), q = w / scale rounded to nearest even within
+ * [-7, 7], 0 where the scale is 0; for finite weights.
+ * sdq_w4_upload copies the packed form (device memory, complete or queued on the default stream;
+ * SDQ_SRC_HOST: host memory) once into the layout of the kernels and returns a handle like those of
+ * sdq_weight_upload (sdq_weight_info, sdq_weight_lookup, sdq_weight_release; the int8 and fp32 entry
+ * points reject it). */
+SDQ_API int sdq_w4_quantize(const void* src_dev, int src_dtype, int64_t N, int64_t K, int group, uint8_t* q_dev,
+                            void* scale_dev, int scale_dtype, uint32_t flags, void* stream);
+SDQ_API int sdq_w4_upload(const uint8_t* q, const void* scale, int scale_dtype, int64_t N, int64_t K, int group,
+                          uint32_t flags, sdq_weight_t* out);
+/* out[M,N] = A[M,K] * W^T (+ bias) (GELU with SDQ_GELU_TANH), for few rows: one token to a small
+ * batch, where the weight's bytes bound a linear.  A is fp32, bf16, fp16, or SDQ_I8 with its row
+ * scales (what sdq_rmsnorm_quantize and sdq_quantize_activations make); out is fp32, bf16 or fp16,
+ * rounded once; bias is fp32 [N] or NULL.  Products and sums keep fp32's precision for every type of
+ * A.  A row of A with a NaN or an infinity gives non-finite outputs in its own row only.  Any M;
+ * beyond a few dozen rows the weights are read again for every 64. */
+SDQ_API int sdq_w4_matmul(sdq_weight_t w, const void* A_dev, int a_dtype, int64_t lda, const float* a_scale_dev,
+                          int64_t M, void* out_dev, int out_dtype, const float* bias_dev, uint32_t flags,
+                          void* stream);
+
+/* A paged int8 key/value cache, in memory that the caller owns.  Each row of head_dim values of one
+ * token and head is kept as head_dim int8 and one fp32 scale (max|x| * (1/127), the recipe of
+ * sdq_rmsnorm_quantize's rows).  head_dim is a multiple of 16 up to 128;
+ * k and v are 16-byte aligned; pages * heads * page_size must fit 31 bits. */
+typedef struct sdq_kv_cache {
+  int8_t* k;       /* [pages, heads, page_size, head_dim] */
+  int8_t* v;
+  float* k_scale;  /* [pages, heads, page_size] */
+  float* v_scale;
+  int64_t pages;
+  int32_t heads, page_size, head_dim, reserved;
+} sdq_kv_cache;
+/* The sequences of a call, in device memory (so that a captured graph sees new lengths).  Rows
+ * [row_start[b], row_start[b+1]) of the call belong to sequence b and are the LAST ones of its
+ * kv_len[b] positions; position p lies in page page_table[b, p / page_size].  row_start does not
+ * decrease; rows in front of row_start[0] and from row_start[batch] on are left alone.  Whatever the
+ * tables hold, no kernel leaves the pool: a position whose page number is not in [0, pages), or that
+ * lies beyond max_pages pages or below zero, is absent -- append drops it, read gives zeros, and
+ * attention does not see it. */
+typedef struct sdq_kv_seqs {
+  const int32_t* row_start;   /* [batch + 1] */
+  const int32_t* kv_len;      /* [batch] */
+  const int32_t* page_table;  /* [batch, max_pages] */
+  int32_t batch, max_pages;
+} sdq_kv_seqs;
+/* Quantizes `rows` rows of keys and values ([rows, heads, head_dim] of dtype, ld elements from row to
+ * row) into the cache; kv_len counts them already.  Pages may be shared between sequences for
+ * reading, but no two rows of a call may fall on one place: which of them stays is not defined. */
+SDQ_API int sdq_kv_append(const sdq_kv_cache* cache, const sdq_kv_seqs* seqs, const void* k_dev,
+                          const void* v_dev, int dtype, int64_t ld, int64_t rows, uint32_t flags,
+                          void* stream);
+/* The way back: the rows that sdq_kv_append with the same arguments wrote, as int8 * scale rounded
+ * once to dtype.  With row_start the running sum of kv_len it reads whole sequences. */
+SDQ_API int sdq_kv_read(const sdq_kv_cache* cache, const sdq_kv_seqs* seqs, void* k_dev, void* v_dev, int dtype,
+                        int64_t ld, int64_t rows, uint32_t flags, void* stream);
+/* out = softmax(scale * q k^T) v over the cache, for each of `heads` query heads (a multiple of the
+ * cache's: query head h reads cache head h / (heads / cache heads)).  q and out are
+ * [rows, heads, head_dim] of dtype.  A row sees all kv_len positions of its sequence, with
+ * SDQ_CAUSAL only those up to its own; one that sees none gives zeros.  One entry point serves single
+ * tokens (row_start = 0, 1, 2, ...) and chunks.  Scores, softmax statistics and sums are fp32; with
+ * fp32 q the products keep 22 bits of every factor. */
+SDQ_API int sdq_kv_attention(const sdq_kv_cache* cache, const sdq_kv_seqs* seqs, const void* q_dev, int dtype,
+                             int64_t ldq, int64_t rows, int heads, float scale, void* out_dev, int64_t ldo,
+                             uint32_t flags, void* stream);
 
 /* The same computation as sdq_qgemm for callers that cannot allocate device memory
  * while they run (a host that has given all HBM to its own pool, a plugin inside

@@ -13,18 +13,13 @@
 #include <climits>
 #include <cstdlib>
 
+#include "quant_common.cuh"
 #include "sdq_internal.h"
 
 namespace sdq {
 namespace {
 
 constexpr int kThreads = 256;
-
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
 
 // Block-wide max of non-negative, non-NaN values.  `red` holds kThreads/32 floats.
 __device__ __forceinline__ float block_max(float v, float* red) {
@@ -37,30 +32,7 @@ __device__ __forceinline__ float block_max(float v, float* red) {
   return warp_max(r);
 }
 
-// |x| folded into a running max the way std::max(mx, fabs(x)) does: a NaN is skipped.
-__device__ __forceinline__ float fold_abs(float mx, float x) { return fmaxf(mx, fabsf(x)); }
-
-// The reference rounds with cvtss2si (src/core/qgemm.cpp:62-69): nearest-even, and
-// INT_MIN for NaN or anything outside 32 bits, then clamps to [-127,127].
-__device__ __forceinline__ int act_round(float p) {
-  int v = (fabsf(p) < 2147483648.0f) ? __float2int_rn(p) : INT_MIN;
-  return max(-127, min(127, v));
-}
-
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-  return (uint32_t)(a & 0xff) | ((uint32_t)(b & 0xff) << 8) | ((uint32_t)(c & 0xff) << 16) |
-         ((uint32_t)(d & 0xff) << 24);
-}
-
 __device__ __forceinline__ float4 ld_stream(const float4* p) { return __ldcs(p); }
-
-// Programmatic dependent launch: lets the GEMM that follows in the stream (launched with
-// the programmatic-serialization attribute) start its prologue -- barrier set-up, tensor
-// memory allocation, descriptor prefetch -- while this kernel is still running.  The GEMM
-// waits (griddepcontrol.wait) for this whole grid and its writes before it reads anything.
-__device__ __forceinline__ void allow_dependent_launch() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
 
 // ---- activations: a row lives in registers between the max and the rounding ----
 // Requires K % 4 == 0, 16-byte aligned A, K <= kThreads * 4 * VPT.
@@ -377,22 +349,6 @@ __global__ void __launch_bounds__(kThreads) ln_mod_quant_regs(const float* __res
 }
 
 // ---- weights ----
-template <int DT>
-__device__ __forceinline__ float load_src(const void* p, int64_t i);
-template <>
-__device__ __forceinline__ float load_src<SDQ_F32>(const void* p, int64_t i) {
-  return static_cast<const float*>(p)[i];
-}
-template <>
-__device__ __forceinline__ float load_src<SDQ_BF16>(const void* p, int64_t i) {
-  // bits << 16, exactly the packer's widening (tools/quantize/pack_sdcpp.py:40-41)
-  return __uint_as_float((uint32_t) static_cast<const uint16_t*>(p)[i] << 16);
-}
-template <>
-__device__ __forceinline__ float load_src<SDQ_F16>(const void* p, int64_t i) {
-  return __half2float(static_cast<const __half*>(p)[i]);  // exact widening
-}
-
 // Round one element under the chosen recipe, given the row's absmax.
 template <int MODE>
 struct RowRecipe {
@@ -426,31 +382,6 @@ struct RowRecipe {
 // One block per row with the row held in registers between the max and the rounding:
 // 16-byte loads (8 bf16/f16 or 4 fp32 elements), packed stores.  Needs last % EPV == 0,
 // 16-byte aligned rows, last <= kThreads * EPV * VPT.
-template <int DT>
-struct Vec {
-  static constexpr int EPV = DT == SDQ_F32 ? 4 : 8;  // elements per 16-byte vector
-  __device__ static void load(const void* row, int idx, float (&v)[EPV]) {
-    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(row) + idx);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    if constexpr (DT == SDQ_F32) {
-#pragma unroll
-      for (int i = 0; i < 4; i++) v[i] = __uint_as_float(w[i]);
-    } else if constexpr (DT == SDQ_BF16) {
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        v[2 * i] = __half2float(__ushort_as_half((unsigned short)(w[i] & 0xffffu)));
-        v[2 * i + 1] = __half2float(__ushort_as_half((unsigned short)(w[i] >> 16)));
-      }
-    }
-  }
-};
-
 template <int DT, int MODE, int VPT>
 __global__ void __launch_bounds__(kThreads) quant_rows_regs(const void* __restrict__ src,
                                                             int64_t rows, int64_t last,

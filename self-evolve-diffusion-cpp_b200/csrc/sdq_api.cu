@@ -10,6 +10,7 @@
 #include <unordered_map>
 #include <vector>
 
+#include "kv_common.cuh"
 #include "sdq_internal.h"
 
 namespace sdq {
@@ -25,6 +26,10 @@ struct Weight {
   // an fp32 weight (sdq_fweight_upload): tf32 planes hi / lo, transposed to [N,K]; q is null
   const float* f_hi = nullptr;
   const float* f_lo = nullptr;
+  // a 4-bit weight (sdq_w4_upload): tiles and group scales in the kernels' layout; q is null
+  const uint32_t* w4 = nullptr;
+  const void* w4_scale = nullptr;
+  int w4_scale_dtype = 0, w4_group = 0;
   bool owned = false;          // q/scale (or f_hi/f_lo) were allocated by the upload
   const void* host_key = nullptr;
   bool live = false;
@@ -137,6 +142,49 @@ WeightRef get_fweight(sdq_weight_t h) {  // an fp32 weight
   WeightRef r = get_any_weight(h);
   r.ok = r.ok && r.w.f_hi != nullptr;
   return r;
+}
+
+WeightRef get_w4_weight(sdq_weight_t h) {  // a 4-bit weight
+  WeightRef r = get_any_weight(h);
+  r.ok = r.ok && r.w.w4 != nullptr;
+  return r;
+}
+
+// Makes the library's GPU current for one call where the calling thread has another one.
+struct DeviceGuard {
+  int prev = -1;
+  int enter() {
+    if (int rc = need_ctx()) return rc;
+    int now = -1;
+    SDQ_CUDA(cudaGetDevice(&now));
+    if (now == g_ctx->device) return SDQ_OK;
+    SDQ_CUDA(cudaSetDevice(g_ctx->device));
+    prev = now;
+    return SDQ_OK;
+  }
+  ~DeviceGuard() { if (prev >= 0) cudaSetDevice(prev); }
+};
+// Body of a C entry point that no exception may leave.
+template <typename F>
+int guarded(F body) {
+  try {
+    return body();
+  } catch (const std::bad_alloc&) {
+    return SDQ_ERR_NOMEM;
+  } catch (...) {
+    return SDQ_ERR_CUDA;
+  }
+}
+int invalid(const char* name, const char* what) { return fail(SDQ_ERR_INVALID, std::string(name) + ": " + what); }
+int launched(const char* name, cudaError_t e, uint32_t flags, void* stream) {
+  if (e != cudaSuccess) return fail(SDQ_ERR_CUDA, std::string(name) + " launch: " + cudaGetErrorString(e));
+  return (flags & SDQ_SYNC) ? sdq_stream_sync(stream) : SDQ_OK;
+}
+bool float_dtype(int t) { return t == SDQ_F32 || t == SDQ_BF16 || t == SDQ_F16; }
+// natural alignment of a typed pointer
+bool natural(const void* p, int dtype) {
+  const uintptr_t mask = dtype == SDQ_F32 ? 3 : dtype == SDQ_I8 ? 0 : 1;
+  return (reinterpret_cast<uintptr_t>(p) & mask) == 0;
 }
 
 int check_status_word() {
@@ -280,6 +328,7 @@ int sdq_shutdown(void) {
     if (w.live && w.owned) {
       cudaFree(const_cast<int8_t*>(w.q)); cudaFree(const_cast<float*>(w.scale));
       cudaFree(const_cast<float*>(w.f_hi)); cudaFree(const_cast<float*>(w.f_lo));
+      cudaFree(const_cast<uint32_t*>(w.w4)); cudaFree(const_cast<void*>(w.w4_scale));
     }
   for (auto& kv : g_ctx->ws) release_workspace(kv.second);
   for (int i = 0; i < 2; i++) {
@@ -509,6 +558,7 @@ int sdq_weight_release(sdq_weight_t h) {
   if (w->owned) {
     cudaFree(const_cast<int8_t*>(w->q)); cudaFree(const_cast<float*>(w->scale));
     cudaFree(const_cast<float*>(w->f_hi)); cudaFree(const_cast<float*>(w->f_lo));
+    cudaFree(const_cast<uint32_t*>(w->w4)); cudaFree(const_cast<void*>(w->w4_scale));
   }
   if (w->host_key) {
     auto it = g_ctx->by_host.find(w->host_key);
@@ -704,6 +754,208 @@ int sdq_sdpa(const float* q_dev, const float* k_dev, const float* v_dev, int64_t
   if (e != cudaSuccess)
     return fail(SDQ_ERR_CUDA, why.empty() ? std::string("attention launch: ") + cudaGetErrorString(e) : why);
   return (flags & SDQ_SYNC) ? sdq_stream_sync(stream) : SDQ_OK;
+}
+
+// ---- RMS norm into int8 rows ----
+int sdq_rmsnorm_quantize(const void* X_dev, int dtype, int64_t ldx, const void* residual_dev, int64_t ldr, int64_t M,
+                         int64_t K, const float* weight_dev, float eps, void* sum_out_dev, int64_t lds, int8_t* aq_dev,
+                         float* a_scale_dev, void* h_out_dev, uint32_t flags, void* stream) {
+  static const char* const kName = "sdq_rmsnorm_quantize";
+  return guarded([&]() -> int {
+    if (M < 0 || K < 0) return invalid(kName, "negative shape");
+    if (!float_dtype(dtype)) return invalid(kName, "dtype must be SDQ_F32, SDQ_BF16 or SDQ_F16");
+    if (flags & ~(uint32_t)SDQ_SYNC) return invalid(kName, "unsupported flag");
+    const bool none = M == 0 || K == 0;
+    if (!none && !X_dev) return invalid(kName, "null pointer");
+    if (!residual_dev != !sum_out_dev) return invalid(kName, "residual and sum_out go together");
+    if (!aq_dev != !a_scale_dev) return invalid(kName, "aq and a_scale go together");
+    if (!none && !aq_dev && !h_out_dev) return invalid(kName, "neither aq nor h_out is asked for");
+    if (!(eps >= 0.0f)) return invalid(kName, "eps must not be negative");
+    const int64_t lx = ldx ? ldx : K, lr = ldr ? ldr : K, ls = lds ? lds : K;
+    if (lx < K || lr < K || ls < K) return invalid(kName, "a row stride is shorter than a row");
+    if (sum_out_dev && ((sum_out_dev == X_dev && ls != lx) || (sum_out_dev == residual_dev && ls != lr)))
+      return invalid(kName, "an in-place sum_out needs its operand's row stride");
+    if (!natural(X_dev, dtype) || !natural(residual_dev, dtype) || !natural(sum_out_dev, dtype) ||
+        !natural(h_out_dev, dtype) || !natural(weight_dev, SDQ_F32) || !natural(a_scale_dev, SDQ_F32))
+      return invalid(kName, "a pointer is not aligned to its element");
+    DeviceGuard g;
+    if (int rc = g.enter()) return rc;
+    if (none) return SDQ_OK;
+    return launched(kName, launch_rmsnorm_quant(X_dev, dtype, lx, residual_dev, lr, M, K, weight_dev, eps, sum_out_dev, ls,
+                                                aq_dev, a_scale_dev, h_out_dev, (cudaStream_t)stream), flags, stream);
+  });
+}
+
+// ---- 4-bit weights ----
+static const char* w4_bad_shape(int64_t N, int64_t K, int group, int scale_dtype) {
+  if (N <= 0 || K <= 0) return "non-positive shape";
+  if (N > (int64_t(1) << 31) - 16 || K > (int64_t(1) << 31) - 128) return "N and K must fit 31 bits";
+  if (group != 32 && group != 64 && group != 128) return "group must be 32, 64 or 128";
+  if (!float_dtype(scale_dtype)) return "scale_dtype must be SDQ_F32, SDQ_BF16 or SDQ_F16";
+  return nullptr;
+}
+
+int sdq_w4_quantize(const void* src_dev, int src_dtype, int64_t N, int64_t K, int group, uint8_t* q_dev, void* scale_dev,
+                    int scale_dtype, uint32_t flags, void* stream) {
+  static const char* const kName = "sdq_w4_quantize";
+  return guarded([&]() -> int {
+    if (const char* bad = w4_bad_shape(N, K, group, scale_dtype)) return invalid(kName, bad);
+    if (!float_dtype(src_dtype)) return invalid(kName, "src_dtype must be SDQ_F32, SDQ_BF16 or SDQ_F16");
+    if (flags & ~(uint32_t)SDQ_SYNC) return invalid(kName, "unsupported flag (device pointers only)");
+    if (!src_dev || !q_dev || !scale_dev) return invalid(kName, "null pointer");
+    if (!natural(src_dev, src_dtype) || !natural(scale_dev, scale_dtype))
+      return invalid(kName, "a pointer is not aligned to its element");
+    DeviceGuard g;
+    if (int rc = g.enter()) return rc;
+    return launched(kName, launch_w4_quantize(src_dev, src_dtype, N, K, group, q_dev, scale_dev, scale_dtype,
+                                              (cudaStream_t)stream), flags, stream);
+  });
+}
+
+int sdq_w4_upload(const uint8_t* q, const void* scale, int scale_dtype, int64_t N, int64_t K, int group, uint32_t flags,
+                  sdq_weight_t* out) {
+  static const char* const kName = "sdq_w4_upload";
+  return guarded([&]() -> int {
+    if (const char* bad = w4_bad_shape(N, K, group, scale_dtype)) return invalid(kName, bad);
+    if (!q || !scale || !out) return invalid(kName, "null pointer");
+    if (flags & ~(uint32_t)SDQ_SRC_HOST) return invalid(kName, "unsupported flag");
+    if (!natural(scale, scale_dtype)) return invalid(kName, "a pointer is not aligned to its element");
+    DeviceGuard g;
+    if (int rc = g.enter()) return rc;
+    const size_t src_bytes = (size_t)N * ((K + 1) / 2), groups = (size_t)((K + group - 1) / group);
+    const size_t src_scale = (size_t)N * groups * (scale_dtype == SDQ_F32 ? 4 : 2);
+    void *stage = nullptr, *stage_scale = nullptr, *dq = nullptr, *ds = nullptr;
+    cudaError_t e = cudaMalloc(&dq, w4_bytes(N, K));
+    if (e == cudaSuccess) e = cudaMalloc(&ds, w4_scale_bytes(N, K, group, scale_dtype));
+    if (flags & SDQ_SRC_HOST) {
+      if (e == cudaSuccess) e = cudaMalloc(&stage, src_bytes);
+      if (e == cudaSuccess) e = cudaMalloc(&stage_scale, src_scale);
+      if (e == cudaSuccess) e = cudaMemcpy(stage, q, src_bytes, cudaMemcpyHostToDevice);
+      if (e == cudaSuccess) e = cudaMemcpy(stage_scale, scale, src_scale, cudaMemcpyHostToDevice);
+    }
+    // on the default stream: after the work queued there (a device source is often its last result),
+    // and complete before the handle is given out
+    if (e == cudaSuccess)
+      e = launch_w4_layout(stage ? (const uint8_t*)stage : q, stage_scale ? stage_scale : scale, scale_dtype, N, K, group,
+                           (uint32_t*)dq, ds, nullptr);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
+    cudaFree(stage); cudaFree(stage_scale);
+    if (e != cudaSuccess) {
+      cudaFree(dq); cudaFree(ds);
+      return fail(e == cudaErrorMemoryAllocation ? SDQ_ERR_NOMEM : SDQ_ERR_CUDA, std::string(kName) + ": " + cudaGetErrorString(e));
+    }
+    Weight w;
+    w.w4 = (const uint32_t*)dq; w.w4_scale = ds; w.w4_scale_dtype = scale_dtype; w.w4_group = group;
+    w.N = N; w.K = K; w.owned = true; w.live = true;
+    if (flags & SDQ_SRC_HOST) w.host_key = q;
+    return register_weight(w, out);
+  });
+}
+
+int sdq_w4_matmul(sdq_weight_t h, const void* A_dev, int a_dtype, int64_t lda, const float* a_scale_dev, int64_t M,
+                  void* out_dev, int out_dtype, const float* bias_dev, uint32_t flags, void* stream) {
+  static const char* const kName = "sdq_w4_matmul";
+  return guarded([&]() -> int {
+    if (M < 0) return invalid(kName, "negative M");
+    if (!float_dtype(a_dtype) && a_dtype != SDQ_I8) return invalid(kName, "a_dtype must be SDQ_F32, SDQ_BF16, SDQ_F16 or SDQ_I8");
+    if (!float_dtype(out_dtype)) return invalid(kName, "out_dtype must be SDQ_F32, SDQ_BF16 or SDQ_F16");
+    if ((a_dtype == SDQ_I8) != (a_scale_dev != nullptr)) return invalid(kName, "a_scale goes with int8 rows, and only with them");
+    if (flags & ~(uint32_t)(SDQ_SYNC | SDQ_GELU_TANH)) return invalid(kName, "unsupported flag (device pointers only)");
+    if (M > 0 && (!A_dev || !out_dev)) return invalid(kName, "null pointer");
+    if (!natural(A_dev, a_dtype) || !natural(out_dev, out_dtype) || !natural(a_scale_dev, SDQ_F32) || !natural(bias_dev, SDQ_F32))
+      return invalid(kName, "a pointer is not aligned to its element");
+    DeviceGuard g;
+    if (int rc = g.enter()) return rc;
+    WeightRef w = get_w4_weight(h);
+    if (!w) return invalid(kName, "bad weight handle (not a 4-bit weight)");
+    if (M == 0) return SDQ_OK;
+    const int64_t ld = lda ? lda : w->K;
+    if (ld < w->K) return invalid(kName, "a row stride is shorter than a row");
+    if (M > INT32_MAX || M * w->N > (int64_t(1) << 33)) return invalid(kName, "M is too large (this is the few-row product)");
+    W4Args a;
+    a.q = w->w4; a.scale = w->w4_scale; a.scale_dtype = w->w4_scale_dtype; a.group = w->w4_group;
+    a.x = A_dev; a.x_dtype = a_dtype; a.ldx = ld; a.x_scale = a_scale_dev; a.bias = bias_dev;
+    a.out = out_dev; a.out_dtype = out_dtype; a.M = M; a.N = w->N; a.K = w->K; a.gelu = (flags & SDQ_GELU_TANH) ? 1 : 0;
+    return launched(kName, launch_w4_matmul(a, (cudaStream_t)stream), flags, stream);
+  });
+}
+
+// ---- paged int8 key/value cache ----
+// Checks the descriptors every entry point takes; fills `a` or says what is wrong.
+static const char* kv_args(const sdq_kv_cache* c, const sdq_kv_seqs* s, int64_t rows, KvArgs* a) {
+  if (!c || !s) return "null descriptor";
+  if (c->pages < 0 || c->heads <= 0 || c->page_size <= 0) return "bad cache shape";
+  if (c->head_dim < 16 || c->head_dim > 128 || c->head_dim % 16 != 0) return "head_dim must be a multiple of 16 up to 128";
+  if (c->heads > (1 << 16) || c->page_size > (1 << 24) || c->pages > INT32_MAX / ((int64_t)c->heads * c->page_size))
+    return "pages * heads * page_size must fit 31 bits";
+  if (s->batch < 0 || s->max_pages < 0 || (int64_t)s->max_pages * c->page_size > INT32_MAX) return "bad sequence table shape";
+  if (rows < 0 || rows > INT32_MAX / 2) return "bad number of rows";
+  if (c->pages > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale)) return "null pointer in the cache";
+  if (s->batch > 0 && (!s->row_start || !s->kv_len || (s->max_pages > 0 && !s->page_table))) return "null pointer in the sequence table";
+  if (((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) != 0) return "the cache's k and v must be 16-byte aligned";
+  if (!natural(c->k_scale, SDQ_F32) || !natural(c->v_scale, SDQ_F32) || !natural(s->row_start, SDQ_F32) ||
+      !natural(s->kv_len, SDQ_F32) || !natural(s->page_table, SDQ_F32))
+    return "a pointer is not aligned to its element";
+  *a = KvArgs{c->k, c->v, c->k_scale, c->v_scale, s->row_start, s->kv_len, s->page_table, PageDiv((uint32_t)c->page_size),
+              (int32_t)c->pages, c->heads, c->page_size, c->head_dim, s->batch, s->max_pages, (int32_t)rows};
+  return nullptr;
+}
+
+static int kv_io(const char* name, const sdq_kv_cache* c, const sdq_kv_seqs* s, void* k, void* v, int dtype, int64_t ld,
+                 int64_t rows, uint32_t flags, void* stream, bool append) {
+  KvArgs a{nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, PageDiv(1), 0, 0, 0, 0, 0, 0, 0};
+  if (const char* bad = kv_args(c, s, rows, &a)) return invalid(name, bad);
+  if (!float_dtype(dtype)) return invalid(name, "dtype must be SDQ_F32, SDQ_BF16 or SDQ_F16");
+  if (flags & ~(uint32_t)SDQ_SYNC) return invalid(name, "unsupported flag");
+  const bool none = rows == 0 || a.batch == 0;
+  if (!none && (!k || !v)) return invalid(name, "null pointer");
+  const int64_t width = (int64_t)a.heads * a.D, l = ld ? ld : width;
+  if (l < width) return invalid(name, "a row stride is shorter than a row");
+  if (!natural(k, dtype) || !natural(v, dtype)) return invalid(name, "a pointer is not aligned to its element");
+  DeviceGuard g;
+  if (int rc = g.enter()) return rc;
+  if (none) return SDQ_OK;
+  return launched(name, launch_kv_io(a, k, v, dtype, l, append, (cudaStream_t)stream), flags, stream);
+}
+
+int sdq_kv_append(const sdq_kv_cache* cache, const sdq_kv_seqs* seqs, const void* k_dev, const void* v_dev, int dtype,
+                  int64_t ld, int64_t rows, uint32_t flags, void* stream) {
+  static const char* const kName = "sdq_kv_append";
+  return guarded([&]() -> int {
+    return kv_io(kName, cache, seqs, const_cast<void*>(k_dev), const_cast<void*>(v_dev), dtype, ld, rows, flags, stream, true);
+  });
+}
+
+int sdq_kv_read(const sdq_kv_cache* cache, const sdq_kv_seqs* seqs, void* k_dev, void* v_dev, int dtype, int64_t ld,
+                int64_t rows, uint32_t flags, void* stream) {
+  static const char* const kName = "sdq_kv_read";
+  return guarded([&]() -> int { return kv_io(kName, cache, seqs, k_dev, v_dev, dtype, ld, rows, flags, stream, false); });
+}
+
+int sdq_kv_attention(const sdq_kv_cache* cache, const sdq_kv_seqs* seqs, const void* q_dev, int dtype, int64_t ldq,
+                     int64_t rows, int heads, float scale, void* out_dev, int64_t ldo, uint32_t flags, void* stream) {
+  static const char* const kName = "sdq_kv_attention";
+  return guarded([&]() -> int {
+    KvArgs a{nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, PageDiv(1), 0, 0, 0, 0, 0, 0, 0};
+    if (const char* bad = kv_args(cache, seqs, rows, &a)) return invalid(kName, bad);
+    if (!float_dtype(dtype)) return invalid(kName, "dtype must be SDQ_F32, SDQ_BF16 or SDQ_F16");
+    if (flags & ~(uint32_t)(SDQ_SYNC | SDQ_CAUSAL)) return invalid(kName, "unsupported flag");
+    if (heads <= 0 || heads % a.heads != 0 || heads > (1 << 16)) return invalid(kName, "heads must be a positive multiple of the cache's heads");
+    if (!(scale > 0.0f) || scale > 1e30f) return invalid(kName, "scale must be positive and finite");
+    if (rows * (int64_t)heads > INT32_MAX) return invalid(kName, "rows * heads must fit 31 bits");
+    const bool none = rows == 0 || a.batch == 0;
+    if (!none && (!q_dev || !out_dev)) return invalid(kName, "null pointer");
+    const int64_t width = (int64_t)heads * a.D;
+    AttendArgs t;
+    t.q = q_dev; t.out = out_dev; t.ldq = ldq ? ldq : width; t.ldo = ldo ? ldo : width;
+    t.heads = heads; t.causal = (flags & SDQ_CAUSAL) ? 1 : 0; t.scale = scale;
+    if (t.ldq < width || t.ldo < width) return invalid(kName, "a row stride is shorter than a row");
+    if (!natural(q_dev, dtype) || !natural(out_dev, dtype)) return invalid(kName, "a pointer is not aligned to its element");
+    DeviceGuard g;
+    if (int rc = g.enter()) return rc;
+    if (none) return SDQ_OK;
+    return launched(kName, launch_kv_attention(a, t, dtype, (cudaStream_t)stream), flags, stream);
+  });
 }
 
 int sdq_qgemm_residual(sdq_weight_t h, const float* A_dev, int64_t M, const float* residual_dev,

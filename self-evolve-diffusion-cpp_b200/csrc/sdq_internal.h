@@ -127,6 +127,36 @@ cudaError_t launch_sdpa(const float* q, const float* k, const float* v, int64_t 
                         int64_t C, int heads, float* out, float* scratch, int* status,
                         uint32_t flags, int sm_count, cudaStream_t s, std::string* why);
 
+// ---- RMS norm + residual + activation quantization: rmsnorm_kernels.cu ----
+// Leading dimensions in elements; residual / sum, weight, aq / a_scale and h may be null (see sdq.h).
+cudaError_t launch_rmsnorm_quant(const void* x, int dtype, int64_t ldx, const void* residual, int64_t ldr, int64_t M,
+                                 int64_t K, const float* weight, float eps, void* sum, int64_t lds, int8_t* aq,
+                                 float* a_scale, void* h, cudaStream_t s);
+
+// ---- 4-bit weights with group scales: w4_kernels.cu ----
+struct W4Args {
+  const uint32_t* q;      // tiles, see w4_kernels.cu
+  const void* scale;
+  int scale_dtype, group;
+  const void* x;          // [M,K], ldx elements from row to row
+  int x_dtype;
+  int64_t ldx;
+  const float* x_scale;   // [M], int8 rows only
+  const float* bias;      // [N] or null
+  void* out;              // [M,N]
+  int out_dtype;
+  int64_t M, N, K;
+  int gelu;
+};
+size_t w4_bytes(int64_t N, int64_t K);
+size_t w4_scale_bytes(int64_t N, int64_t K, int group, int scale_dtype);
+cudaError_t launch_w4_quantize(const void* src, int src_dtype, int64_t N, int64_t K, int group, uint8_t* q, void* scale,
+                               int scale_dtype, cudaStream_t s);
+// packed rows (low nibble first) + scales [N, groups], device memory, into the tile layout
+cudaError_t launch_w4_layout(const uint8_t* q, const void* scale, int scale_dtype, int64_t N, int64_t K, int group,
+                             uint32_t* q_out, void* scale_out, cudaStream_t s);
+cudaError_t launch_w4_matmul(const W4Args& a, cudaStream_t s);
+
 // MMA-issue-bound int8 rate of the device (mma_probe.cu).
 int int8_mma_probe(int sm_count, int iters, int* status_dev, double* seconds, double* ops);
 int wait_expiry_selftest(int limit_ms, int code, int* status_dev, int* outcome_dev, cudaStream_t s);

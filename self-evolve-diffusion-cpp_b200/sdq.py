@@ -15,7 +15,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 A_HOST, OUT_HOST, GELU_TANH, FORCE_SIMT, SYNC, LN_TREE_SUMS, LN_AFFINE = 0x1, 0x2, 0x4, 0x8, 0x10, 0x20, 0x40
 SDPA_V_FP16 = 0x80
 SDPA_K_FP16 = 0x100
-F32, BF16, F16 = 0, 1, 2
+CAUSAL = 0x200
+F32, BF16, F16, I8 = 0, 1, 2, 3
 MODE_PACKER, MODE_ROWWISE = 0, 1
 SRC_HOST, DST_HOST = 0x1, 0x2
 PACK_UPLOAD = 0x1
@@ -49,6 +50,19 @@ class Entry(C.Structure):
     _fields_ = [("name", C.c_void_p), ("dtype", C.c_int32), ("ndim", C.c_int32),
                 ("dims", C.c_int64 * 8), ("data", C.c_void_p), ("nbytes", C.c_uint64),
                 ("file_offset", C.c_uint64), ("weight", C.c_uint64), ("name_len", C.c_uint64)]
+
+
+class KvCache(C.Structure):
+    """sdq_kv_cache: device addresses of the caller's pool."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("pages", C.c_int64), ("heads", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32),
+                ("reserved", C.c_int32)]
+
+
+class KvSeqs(C.Structure):
+    """sdq_kv_seqs: device addresses of the tables that say which rows belong to which sequence."""
+    _fields_ = [("row_start", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p),
+                ("batch", C.c_int32), ("max_pages", C.c_int32)]
 
 
 _SIGS = {
@@ -93,6 +107,21 @@ _SIGS = {
     "sdq_fmatmul": (C.c_int, [C.c_uint64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p]),
     "sdq_sdpa": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int,
                            C.c_void_p, C.c_uint32, C.c_void_p]),
+    "sdq_rmsnorm_quantize": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64,
+                                       C.c_void_p, C.c_float, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p,
+                                       C.c_void_p, C.c_uint32, C.c_void_p]),
+    "sdq_w4_quantize": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_int,
+                                  C.c_uint32, C.c_void_p]),
+    "sdq_w4_upload": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int, C.c_uint32,
+                                C.POINTER(C.c_uint64)]),
+    "sdq_w4_matmul": (C.c_int, [C.c_uint64, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int,
+                                C.c_void_p, C.c_uint32, C.c_void_p]),
+    "sdq_kv_append": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvSeqs), C.c_void_p, C.c_void_p, C.c_int, C.c_int64,
+                                C.c_int64, C.c_uint32, C.c_void_p]),
+    "sdq_kv_read": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvSeqs), C.c_void_p, C.c_void_p, C.c_int, C.c_int64,
+                              C.c_int64, C.c_uint32, C.c_void_p]),
+    "sdq_kv_attention": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvSeqs), C.c_void_p, C.c_int, C.c_int64, C.c_int64,
+                                   C.c_int, C.c_float, C.c_void_p, C.c_int64, C.c_uint32, C.c_void_p]),
     "sdq_qgemm_residual": (C.c_int, [C.c_uint64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
                                      C.c_void_p, C.c_uint32, C.c_void_p]),
     "sdq_ffn_block": (C.c_int, [C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p, C.c_int64,
@@ -448,7 +477,55 @@ class Sdq:
         self._ck(self.lib.sdq_qgemm_static_scratch(wq_ptr, ws_ptr, N, K, A_ptr, M, out_ptr, bias_ptr,
                                                    flags, stream))
 
+    # ---- few-bit inference: raw device pointers ----
+    def rmsnorm_quantize(self, X_ptr, dtype, M, K, aq_ptr, a_scale_ptr, weight_ptr=None, eps=1e-6, residual_ptr=None,
+                         sum_ptr=None, h_ptr=None, ldx=0, ldr=0, lds=0, flags=0, stream=None):
+        """[residual +] RMS norm -> int8 rows and scales (and / or h)."""
+        self._ck(self.lib.sdq_rmsnorm_quantize(X_ptr, dtype, ldx, residual_ptr, ldr, M, K, weight_ptr, eps, sum_ptr, lds,
+                                               aq_ptr, a_scale_ptr, h_ptr, flags, stream))
+
+    def w4_quantize(self, src_ptr, src_dtype, N, K, group, q_ptr, scale_ptr, scale_dtype, flags=0, stream=None):
+        """[N,K] on the device -> packed nibbles [N, ceil(K/2)] and scales [N, ceil(K/group)]."""
+        self._ck(self.lib.sdq_w4_quantize(src_ptr, src_dtype, N, K, group, q_ptr, scale_ptr, scale_dtype, flags, stream))
+
+    def w4_upload(self, q_ptr, scale_ptr, scale_dtype, N, K, group, flags=0):
+        """Packed 4-bit weight (device pointers; host pointers with SRC_HOST) -> handle for w4_matmul."""
+        h = C.c_uint64(0)
+        self._ck(self.lib.sdq_w4_upload(q_ptr, scale_ptr, scale_dtype, N, K, group, flags, C.byref(h)))
+        return h.value
+
+    def w4_matmul(self, w, A_ptr, a_dtype, M, out_ptr, out_dtype=F32, a_scale_ptr=None, bias_ptr=None, gelu=False, lda=0,
+                  flags=0, stream=None):
+        """out[M,N] = A W^T (+ bias) (GELU) with a 4-bit weight."""
+        self._ck(self.lib.sdq_w4_matmul(w, A_ptr, a_dtype, lda, a_scale_ptr, M, out_ptr, out_dtype, bias_ptr,
+                                        flags | (GELU_TANH if gelu else 0), stream))
+
+    def kv_cache(self, k_ptr, v_ptr, k_scale_ptr, v_scale_ptr, pages, heads, page_size, head_dim):
+        """Descriptor of a paged int8 cache over the caller's device buffers."""
+        return KvCache(k_ptr, v_ptr, k_scale_ptr, v_scale_ptr, pages, heads, page_size, head_dim, 0)
+
+    def kv_seqs(self, row_start_ptr, kv_len_ptr, page_table_ptr, batch, max_pages):
+        """Descriptor of the sequences of a call (int32 tables on the device)."""
+        return KvSeqs(row_start_ptr, kv_len_ptr, page_table_ptr, batch, max_pages)
+
+    def kv_append(self, cache, seqs, k_ptr, v_ptr, dtype, rows, ld=0, flags=0, stream=None):
+        self._ck(self.lib.sdq_kv_append(cache, seqs, k_ptr, v_ptr, dtype, ld, rows, flags, stream))
+
+    def kv_read(self, cache, seqs, k_ptr, v_ptr, dtype, rows, ld=0, flags=0, stream=None):
+        self._ck(self.lib.sdq_kv_read(cache, seqs, k_ptr, v_ptr, dtype, ld, rows, flags, stream))
+
+    def kv_attention(self, cache, seqs, q_ptr, dtype, rows, heads, out_ptr, scale=None, causal=False, ldq=0, ldo=0,
+                     flags=0, stream=None):
+        """softmax(scale q k^T) v over the cache; scale defaults to 1 / sqrt(head_dim)."""
+        self._ck(self.lib.sdq_kv_attention(cache, seqs, q_ptr, dtype, ldq, rows, heads,
+                                           cache.head_dim ** -0.5 if scale is None else scale, out_ptr, ldo,
+                                           flags | (CAUSAL if causal else 0), stream))
+
     # ---- quantizers ----
+    def dequant_rows_device(self, q_ptr, scale_ptr, rows, last, w_ptr, flags=0, stream=None):
+        """Raw call of sdq_dequant_rows: device pointers unless SRC_HOST / DST_HOST."""
+        self._ck(self.lib.sdq_dequant_rows(q_ptr, scale_ptr, rows, last, w_ptr, flags, stream))
+
     def quantize_rows(self, src, src_dtype, mode):
         """src: numpy [rows,last] of float32 (F32) or uint16 bit patterns (BF16/F16)."""
         src = np.ascontiguousarray(src)
