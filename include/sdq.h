@@ -357,7 +357,7 @@ SDQ_API int sdq_w4_upload(const uint8_t* q, const void* scale, int scale_dtype, 
  * scales (what sdq_rmsnorm_quantize and sdq_quantize_activations make); out is fp32, bf16 or fp16,
  * rounded once; bias is fp32 [N] or NULL.  Products and sums keep fp32's precision for every type of
  * A.  A row of A with a NaN or an infinity gives non-finite outputs in its own row only.  Any M;
- * beyond a few dozen rows the weights are read again for every 64. */
+ * the weights are read again (from L2 where they fit) for every 8 rows. */
 SDQ_API int sdq_w4_matmul(sdq_weight_t w, const void* A_dev, int a_dtype, int64_t lda, const float* a_scale_dev,
                           int64_t M, void* out_dev, int out_dtype, const float* bias_dev, uint32_t flags,
                           void* stream);

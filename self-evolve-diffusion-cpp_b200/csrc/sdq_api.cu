@@ -26,9 +26,8 @@ struct Weight {
   // an fp32 weight (sdq_fweight_upload): tf32 planes hi / lo, transposed to [N,K]; q is null
   const float* f_hi = nullptr;
   const float* f_lo = nullptr;
-  // a 4-bit weight (sdq_w4_upload): tiles and group scales in the kernels' layout; q is null
+  // a 4-bit weight (sdq_w4_upload): tiles with their scales in the kernels' layout; q is null
   const uint32_t* w4 = nullptr;
-  const void* w4_scale = nullptr;
   int w4_scale_dtype = 0, w4_group = 0;
   bool owned = false;          // q/scale (or f_hi/f_lo) were allocated by the upload
   const void* host_key = nullptr;
@@ -328,7 +327,7 @@ int sdq_shutdown(void) {
     if (w.live && w.owned) {
       cudaFree(const_cast<int8_t*>(w.q)); cudaFree(const_cast<float*>(w.scale));
       cudaFree(const_cast<float*>(w.f_hi)); cudaFree(const_cast<float*>(w.f_lo));
-      cudaFree(const_cast<uint32_t*>(w.w4)); cudaFree(const_cast<void*>(w.w4_scale));
+      cudaFree(const_cast<uint32_t*>(w.w4));
     }
   for (auto& kv : g_ctx->ws) release_workspace(kv.second);
   for (int i = 0; i < 2; i++) {
@@ -558,7 +557,7 @@ int sdq_weight_release(sdq_weight_t h) {
   if (w->owned) {
     cudaFree(const_cast<int8_t*>(w->q)); cudaFree(const_cast<float*>(w->scale));
     cudaFree(const_cast<float*>(w->f_hi)); cudaFree(const_cast<float*>(w->f_lo));
-    cudaFree(const_cast<uint32_t*>(w->w4)); cudaFree(const_cast<void*>(w->w4_scale));
+    cudaFree(const_cast<uint32_t*>(w->w4));
   }
   if (w->host_key) {
     auto it = g_ctx->by_host.find(w->host_key);
@@ -824,9 +823,8 @@ int sdq_w4_upload(const uint8_t* q, const void* scale, int scale_dtype, int64_t 
     if (int rc = g.enter()) return rc;
     const size_t src_bytes = (size_t)N * ((K + 1) / 2), groups = (size_t)((K + group - 1) / group);
     const size_t src_scale = (size_t)N * groups * (scale_dtype == SDQ_F32 ? 4 : 2);
-    void *stage = nullptr, *stage_scale = nullptr, *dq = nullptr, *ds = nullptr;
-    cudaError_t e = cudaMalloc(&dq, w4_bytes(N, K));
-    if (e == cudaSuccess) e = cudaMalloc(&ds, w4_scale_bytes(N, K, group, scale_dtype));
+    void *stage = nullptr, *stage_scale = nullptr, *dq = nullptr;
+    cudaError_t e = cudaMalloc(&dq, w4_bytes(N, K, group, scale_dtype));
     if (flags & SDQ_SRC_HOST) {
       if (e == cudaSuccess) e = cudaMalloc(&stage, src_bytes);
       if (e == cudaSuccess) e = cudaMalloc(&stage_scale, src_scale);
@@ -837,15 +835,15 @@ int sdq_w4_upload(const uint8_t* q, const void* scale, int scale_dtype, int64_t 
     // and complete before the handle is given out
     if (e == cudaSuccess)
       e = launch_w4_layout(stage ? (const uint8_t*)stage : q, stage_scale ? stage_scale : scale, scale_dtype, N, K, group,
-                           (uint32_t*)dq, ds, nullptr);
+                           (uint32_t*)dq, nullptr);
     if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
     cudaFree(stage); cudaFree(stage_scale);
     if (e != cudaSuccess) {
-      cudaFree(dq); cudaFree(ds);
+      cudaFree(dq);
       return fail(e == cudaErrorMemoryAllocation ? SDQ_ERR_NOMEM : SDQ_ERR_CUDA, std::string(kName) + ": " + cudaGetErrorString(e));
     }
     Weight w;
-    w.w4 = (const uint32_t*)dq; w.w4_scale = ds; w.w4_scale_dtype = scale_dtype; w.w4_group = group;
+    w.w4 = (const uint32_t*)dq; w.w4_scale_dtype = scale_dtype; w.w4_group = group;
     w.N = N; w.K = K; w.owned = true; w.live = true;
     if (flags & SDQ_SRC_HOST) w.host_key = q;
     return register_weight(w, out);
@@ -873,7 +871,7 @@ int sdq_w4_matmul(sdq_weight_t h, const void* A_dev, int a_dtype, int64_t lda, c
     if (ld < w->K) return invalid(kName, "a row stride is shorter than a row");
     if (M > INT32_MAX || M * w->N > (int64_t(1) << 33)) return invalid(kName, "M is too large (this is the few-row product)");
     W4Args a;
-    a.q = w->w4; a.scale = w->w4_scale; a.scale_dtype = w->w4_scale_dtype; a.group = w->w4_group;
+    a.q = w->w4; a.scale_dtype = w->w4_scale_dtype; a.group = w->w4_group;
     a.x = A_dev; a.x_dtype = a_dtype; a.ldx = ld; a.x_scale = a_scale_dev; a.bias = bias_dev;
     a.out = out_dev; a.out_dtype = out_dtype; a.M = M; a.N = w->N; a.K = w->K; a.gelu = (flags & SDQ_GELU_TANH) ? 1 : 0;
     return launched(kName, launch_w4_matmul(a, (cudaStream_t)stream), flags, stream);

@@ -135,8 +135,7 @@ cudaError_t launch_rmsnorm_quant(const void* x, int dtype, int64_t ldx, const vo
 
 // ---- 4-bit weights with group scales: w4_kernels.cu ----
 struct W4Args {
-  const uint32_t* q;      // tiles, see w4_kernels.cu
-  const void* scale;
+  const uint32_t* q;      // tiles with their scales, see w4_kernels.cu
   int scale_dtype, group;
   const void* x;          // [M,K], ldx elements from row to row
   int x_dtype;
@@ -148,13 +147,12 @@ struct W4Args {
   int64_t M, N, K;
   int gelu;
 };
-size_t w4_bytes(int64_t N, int64_t K);
-size_t w4_scale_bytes(int64_t N, int64_t K, int group, int scale_dtype);
+size_t w4_bytes(int64_t N, int64_t K, int group, int scale_dtype);
 cudaError_t launch_w4_quantize(const void* src, int src_dtype, int64_t N, int64_t K, int group, uint8_t* q, void* scale,
                                int scale_dtype, cudaStream_t s);
 // packed rows (low nibble first) + scales [N, groups], device memory, into the tile layout
 cudaError_t launch_w4_layout(const uint8_t* q, const void* scale, int scale_dtype, int64_t N, int64_t K, int group,
-                             uint32_t* q_out, void* scale_out, cudaStream_t s);
+                             uint32_t* out, cudaStream_t s);
 cudaError_t launch_w4_matmul(const W4Args& a, cudaStream_t s);
 
 // MMA-issue-bound int8 rate of the device (mma_probe.cu).

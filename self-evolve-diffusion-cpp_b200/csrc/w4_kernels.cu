@@ -3,24 +3,29 @@
 //   w[n,k] = sc[n, k/g] * q[n,k],  q in [-8, 7]
 //   y[m,n] = sum_G sc[n,G] * sum_{k in G} a[m,k] q[n,k]   (* a_scale[m] for int8 rows, + bias, GELU)
 //
-// Layout of an uploaded weight: tiles of 16 rows x 64 columns, 512 bytes each, the tiles of 16 rows
-// one after the other along k.  Lane 4 g + c of a warp owns 16 bytes of a tile: word j holds its share
-// of columns 16 j .. 16 j + 15, nibbles (0,4) row g columns 2c, 2c+1; (1,5) row g + 8, the same
-// columns; (2,6) row g, columns 2c + 8, 2c + 9; (3,7) row g + 8 of those.  A nibble is q + 8; rows and
-// columns beyond the matrix hold 8 (zero).  Scales lie as [16-row tile][group][16].
+// Layout of an uploaded weight: tiles of 16 rows x 128 columns, 1 KB and their scales, the tiles of 16 rows one
+// after the other along k.  Lane 4 g + c of a warp owns two pieces of 16 bytes, 512 apart, for 64
+// columns each: words 2 i and 2 i + 1 of a piece hold its share of columns 32 i .. 32 i + 31, which is
+// columns 8c .. 8c + 7 of rows g and g + 8.  Nibbles (0,4) are row g, columns 8c + 4h, + 1 of word
+// 2 i + h; (1,5) row g + 8, the same columns; (2,6) row g, columns 8c + 4h + 2, + 3; (3,7) row g + 8 of
+// those.  A nibble is q + 8; rows and columns beyond the matrix hold 8 (zero).  The scales of a tile
+// follow its weights, [group][row % 8][row / 8]: a tile is one run of memory.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
 #include "epilogue.cuh"
 #include "quant_common.cuh"
 #include "sdq_internal.h"
+
+namespace cg = cooperative_groups;
 
 namespace sdq {
 namespace {
 
 constexpr int kBlock = 256;
 
-template <int DT>
-__device__ __forceinline__ float scale_at(const void* p, int64_t i) { return load_src<DT>(p, i); }
-
-// ---- quantizer: one thread per 8 columns... one warp per (row, group) ----
+// ---- quantizer: a warp per (row, group) ----
 template <int DT, int ST>
 __global__ void __launch_bounds__(kBlock) w4_quantize_kernel(const void* __restrict__ src, int64_t N, int64_t K,
                                                              int group, uint8_t* __restrict__ q, void* __restrict__ scale) {
@@ -58,70 +63,499 @@ __global__ void __launch_bounds__(kBlock) w4_quantize_kernel(const void* __restr
   }
 }
 
-// ---- upload: [N, ceil(K/2)] bytes, low nibble first, into the tiles ----
-__global__ void __launch_bounds__(kBlock) w4_layout_kernel(const uint8_t* __restrict__ q, int64_t N, int64_t K,
-                                                           int64_t words, uint32_t* __restrict__ out) {
-  const int64_t row_bytes = (K + 1) / 2, k_tiles = (K + 63) / 64;
+// Bytes of a tile.
+__host__ __device__ constexpr int kTileBytes(int ss, int group) { return 1024 + 128 / group * 16 * ss; }
+
+// ---- upload: [N, ceil(K/2)] bytes, low nibble first, and [N, groups] scales into the tiles ----
+// `tile_words` 32-bit words a tile; SIZE bytes a scale.
+template <int SIZE>
+__global__ void __launch_bounds__(kBlock) w4_layout_kernel(const uint8_t* __restrict__ q, const void* __restrict__ scale, int64_t N,
+                                                           int64_t K, int group, int tile_words, int64_t words,
+                                                           uint32_t* __restrict__ out) {
+  const int64_t row_bytes = (K + 1) / 2, k_tiles = (K + 127) / 128, groups = (K + group - 1) / group;
   for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < words; i += (int64_t)gridDim.x * kBlock) {
-    const int j = (int)(i & 3), lane = (int)(i >> 2) & 31;
-    const int64_t tile = i >> 7, nt = tile / k_tiles, kt = tile - nt * k_tiles;
+    const int64_t tile = i / tile_words, nt = tile / k_tiles, kt = tile - nt * k_tiles;
+    const int at = (int)(i - tile * tile_words);
     uint32_t w = 0;
+    if (at < 256) {
+      const int j = at & 3, lane = (at >> 2) & 31, piece = at >> 7;
 #pragma unroll
-    for (int p = 0; p < 8; p++) {
-      const int64_t n = nt * 16 + (lane >> 2) + 8 * (p & 1);
-      const int64_t k = kt * 64 + j * 16 + 2 * (lane & 3) + 8 * ((p >> 1) & 1) + (p >> 2);
-      uint32_t v = 8;
-      if (n < N && k < K) v = (q[n * row_bytes + (k >> 1)] >> (4 * (k & 1))) & 15u;
-      w |= v << (4 * p);
+      for (int p = 0; p < 8; p++) {
+        const int64_t n = nt * 16 + (lane >> 2) + 8 * (p & 1);
+        const int64_t k = kt * 128 + piece * 64 + (j >> 1) * 32 + 8 * (lane & 3) + 4 * (j & 1) + 2 * ((p >> 1) & 1) + (p >> 2);
+        uint32_t v = 8;
+        if (n < N && k < K) v = (q[n * row_bytes + (k >> 1)] >> (4 * (k & 1))) & 15u;
+        w |= v << (4 * p);
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 4 / SIZE; h++) {
+        const int e = (at - 256) * (4 / SIZE) + h;   // scale of the tile: [group][row % 8][row / 8]
+        const int64_t n = nt * 16 + ((e & 15) >> 1) + 8 * (e & 1), g = kt * (128 / group) + (e >> 4);
+        if (n < N && g < groups) {
+          if constexpr (SIZE == 4) w = static_cast<const uint32_t*>(scale)[n * groups + g];
+          else w |= (uint32_t) static_cast<const uint16_t*>(scale)[n * groups + g] << (16 * h);
+        }
+      }
     }
     out[i] = w;
   }
 }
-template <int SIZE>
-__global__ void __launch_bounds__(kBlock) w4_scale_layout_kernel(const void* __restrict__ src, int64_t N, int64_t groups,
-                                                                 int64_t count, void* __restrict__ out) {
-  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < count; i += (int64_t)gridDim.x * kBlock) {
-    const int64_t n = (i >> 4) / groups * 16 + (i & 15), g = (i >> 4) % groups;
-    if constexpr (SIZE == 4)
-      static_cast<uint32_t*>(out)[i] = n < N ? static_cast<const uint32_t*>(src)[n * groups + g] : 0u;
-    else
-      static_cast<uint16_t*>(out)[i] = n < N ? static_cast<const uint16_t*>(src)[n * groups + g] : (uint16_t)0;
+
+// ---- products ----
+// A warp owns 16 weight rows and streams their tiles; a tile is one 16-byte load of each lane.  The
+// nibbles become fp16 (or bf16) integers in registers, which are the A operand of m16n8k16 tensor
+// instructions; the activations, 8 rows of x to an instruction, are the B operand.  Sums of 64 columns
+// (32 with groups of 32) stay in the accumulators and leave them by one fused multiply-add with the
+// group's scale.
+//
+// Exactness: q is an integer of 4 bits, exact in either 16-bit type.  fp16 and int8 rows enter as fp16
+// and bf16 rows as bf16, as they are; fp32 rows as two fp16 numbers (hi + lo, 22 bits) times a power of
+// two for each row and slice.  int8 sums are whole numbers below 2^24 and exact.
+__device__ __forceinline__ uint32_t lop3_and_or(uint32_t a, uint32_t mask, uint32_t or_) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(mask), "r"(or_));   // (a & mask) | or_
+  return r;
+}
+template <bool BF>
+__device__ __forceinline__ void nibbles_to_16(uint32_t w, uint32_t (&a)[4]) {
+  if constexpr (BF) {
+    // 0x4300 is 128 with a last place of 1: 128 + v is exact, and so is the difference from 136
+    const __nv_bfloat162 off = __floats2bfloat162_rn(136.0f, 136.0f);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t t = lop3_and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
+      const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&t), off);
+      a[i] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+  } else {
+    // 0x6400 is 1024 with a last place of 1: 1024 + v or 1024 + 16 v, then v - 8 by one exact operation
+    const __half2 off = __floats2half2_rn(1032.0f, 1032.0f), sixteenth = __floats2half2_rn(0.0625f, 0.0625f),
+                  off16 = __floats2half2_rn(-72.0f, -72.0f);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const uint32_t t = lop3_and_or(w >> (8 * i), 0x000f000fu, 0x64006400u);
+      const uint32_t u = lop3_and_or(w >> (8 * i), 0x00f000f0u, 0x64006400u);
+      const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&t), off);
+      const __half2 s = __hfma2(*reinterpret_cast<const __half2*>(&u), sixteenth, off16);
+      a[2 * i] = *reinterpret_cast<const uint32_t*>(&r);
+      a[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&s);
+    }
+  }
+}
+template <bool BF, bool FIRST>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
+#define SDQ_MMA(TYPE, C0, C1, C2, C3)                                                                              \
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, " \
+               "{%10,%11,%12,%13};"                                                                                \
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                                    \
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(C0), "f"(C1), "f"(C2), "f"(C3))
+  if constexpr (BF && FIRST) SDQ_MMA("bf16", 0.0f, 0.0f, 0.0f, 0.0f);
+  else if constexpr (BF) SDQ_MMA("bf16", c[0], c[1], c[2], c[3]);
+  else if constexpr (FIRST) SDQ_MMA("f16", 0.0f, 0.0f, 0.0f, 0.0f);
+  else SDQ_MMA("f16", c[0], c[1], c[2], c[3]);
+#undef SDQ_MMA
+}
+// Asynchronous 16-byte copies into shared memory.
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Scales of rows g and g + 8, stored side by side.
+template <int ST>
+__device__ __forceinline__ float2 scale_pair(const uint8_t* p) {
+  if constexpr (ST == SDQ_F32) {
+    return *reinterpret_cast<const float2*>(p);
+  } else if constexpr (ST == SDQ_BF16) {
+    const uint32_t v = *reinterpret_cast<const uint32_t*>(p);
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  } else {
+    return __half22float2(*reinterpret_cast<const __half2*>(p));
   }
 }
 
-__device__ __forceinline__ float any_scale(const void* p, int64_t i, int dt) {
-  return dt == SDQ_F32 ? load_src<SDQ_F32>(p, i) : dt == SDQ_BF16 ? load_src<SDQ_BF16>(p, i) : load_src<SDQ_F16>(p, i);
+// How a launch is cut.  A cluster of `ck` blocks owns `strip` (or one less) 16-row tiles of the weight;
+// its blocks split k, `slice` tiles of 128 columns each.  A block keeps its slice of x in shared memory,
+// in stages of `stage` tiles where it does not fit, and deals the (row tile, k tile) pairs of a stage out
+// to its warps in contiguous runs: every warp streams the same number of weight bytes, without a pause at
+// the end of a row tile, and a row tile that crosses warps is summed afterwards.
+struct W4Plan {
+  int ck, strips_long, strip, slice, stage, slots;
+  int x, red, part;   // offsets in shared memory, in bytes
+};
+
+constexpr int kWarps = kBlock / 32;
+constexpr int kRows = 8;    // rows of x to a block
+// Weight tiles that a warp has under way.  Loads into registers do not get that far: the hardware
+// counts them in six classes, so a wait for an old one is a wait for younger ones too.
+constexpr int kAhead = 4;
+constexpr int kBlocksPerSm = 2;
+// n values of x from column k on; zeros behind the end of the row.
+template <int XT>
+__device__ __forceinline__ void x_scalars(const W4Args& a, int64_t row, int k, int n, float* v) {
+  for (int j = 0; j < n; j++) {
+    float f = 0.0f;
+    if (k + j < a.K) {
+      if constexpr (XT == SDQ_I8) f = (float)static_cast<const int8_t*>(a.x)[row * a.ldx + k + j];
+      else f = load_src<XT>(a.x, row * a.ldx + k + j);
+    }
+    v[j] = f;
+  }
 }
-__device__ __forceinline__ float any_act(const void* p, int64_t i, int dt) {
-  return dt == SDQ_I8 ? (float)static_cast<const int8_t*>(p)[i] : any_scale(p, i, dt);
+__device__ __forceinline__ uint32_t half2_bits(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// One warp per output: lanes along k.
-__global__ void __launch_bounds__(kBlock) w4_simple_kernel(const W4Args a) {
-  wait_prior_grids();
-  const int lane = threadIdx.x & 31;
-  const int64_t i = (int64_t)blockIdx.x * (kBlock / 32) + (threadIdx.x >> 5);
-  if (i >= a.M * a.N) return;
-  const int64_t m = i / a.N, n = i - m * a.N;
-  const int64_t k_tiles = (a.K + 63) / 64, groups = (a.K + a.group - 1) / a.group;
-  const int64_t nt = n >> 4;
-  const int r = (int)(n & 15);
-  float y = 0.0f;
-  for (int64_t k = lane; k < a.K; k += 32) {
-    const int kk = (int)(k & 15);
-    const int64_t word = ((nt * k_tiles + (k >> 6)) * 32 + (r & 7) * 4 + ((kk & 7) >> 1)) * 4 + ((k >> 4) & 3);
-    const int p = (r >> 3) + 2 * (kk >> 3) + 4 * (kk & 1);
-    const float q = (float)((int)((a.q[word] >> (4 * p)) & 15u) - 8);
-    y = fmaf(any_act(a.x, m * a.ldx + k, a.x_dtype) * q, any_scale(a.scale, (nt * groups + k / a.group) * 16 + r, a.scale_dtype), y);
+// x of columns [k0, k0 + 128 tiles) into shared memory as [k32][plane][row][32], 16-bit elements.
+template <int XT>
+__device__ __forceinline__ void fill_x(const W4Args& a, int m0, int rows, int k0, int tiles, int vec, uint8_t* smem,
+                                       float* row_exp) {
+  auto floats4 = [&](int r, int k, float (&f)[4]) {
+    if (vec) {
+      const float4 q = k < a.K ? __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.x) + (m0 + r) * a.ldx + k))
+                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      f[0] = q.x; f[1] = q.y; f[2] = q.z; f[3] = q.w;
+    } else {
+      x_scalars<XT>(a, m0 + r, k, 4, f);
+    }
+  };
+  if constexpr (XT == SDQ_F32) {
+    // largest finite |x| of each row into [2^14, 2^15): fp16 holds it, and lo's last place lies 2^-39
+    // below it
+    const int parts = kWarps / rows, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if ((int)threadIdx.x < rows) row_exp[threadIdx.x] = 0.0f;
+    __syncthreads();
+    const int nv = tiles * 32;
+    if (warp < rows * parts) {
+      const int r = warp % rows, part = warp / rows;
+      float mx = 0.0f;
+#pragma unroll 4
+      for (int v = part * 32 + lane; v < nv; v += 32 * parts) {
+        float f[4];
+        floats4(r, k0 + v * 4, f);
+#pragma unroll
+        for (int e = 0; e < 4; e++) mx = fabsf(f[e]) <= 3.402823466e38f ? fmaxf(mx, fabsf(f[e])) : mx;
+      }
+      mx = warp_max(mx);
+      if (lane == 0) atomicMax(reinterpret_cast<int*>(row_exp) + r, __float_as_int(mx));   // order of positive floats
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < rows) {
+      const float mx = row_exp[threadIdx.x];
+      const int e = max(mx > 0.0f ? ilogbf(mx) - 14 : 0, -126);
+      row_exp[threadIdx.x] = __uint_as_float((uint32_t)(e + 127) << 23);   // 2^e, e in -126..113
+    }
+    __syncthreads();
+    uint2* dst = reinterpret_cast<uint2*>(smem);
+#pragma unroll 2
+    for (int i = threadIdx.x; i < nv * rows; i += kBlock) {
+      const int r = i / nv, v = i - r * nv;
+      float f[4];
+      floats4(r, k0 + v * 4, f);
+      const float inv = __uint_as_float((254u << 23) - __float_as_uint(row_exp[r]));   // 2^-e, exact
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const float p = f[2 * e] * inv, q = f[2 * e + 1] * inv;
+        hi[e] = half2_bits(p, q);
+        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+        lo[e] = half2_bits(isinf(back.x) ? 0.0f : p - back.x, isinf(back.y) ? 0.0f : q - back.y);   // an infinity has no rest
+      }
+      const int at = ((v >> 3) * 2 * rows + r) * 8 + (v & 7);
+      dst[at] = make_uint2(hi[0], hi[1]);
+      dst[at + rows * 8] = make_uint2(lo[0], lo[1]);
+    }
+  } else if constexpr (XT == SDQ_I8) {
+    const int nv = tiles * 8;
+    uint4* dst = reinterpret_cast<uint4*>(smem);
+#pragma unroll 2
+    for (int i = threadIdx.x; i < nv * rows; i += kBlock) {
+      const int r = i / nv, v = i - r * nv, k = k0 + v * 16;
+      float f[16];
+      if (vec) {
+        const uint4 q = k < a.K ? __ldg(reinterpret_cast<const uint4*>(static_cast<const int8_t*>(a.x) + (m0 + r) * a.ldx + k))
+                                : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int e = 0; e < 16; e++) f[e] = (float)(int8_t)(w[e >> 2] >> (8 * (e & 3)));
+      } else {
+        x_scalars<XT>(a, m0 + r, k, 16, f);
+      }
+      uint32_t h[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) h[e] = half2_bits(f[2 * e], f[2 * e + 1]);
+      const int at = ((v >> 1) * rows + r) * 4 + (v & 1) * 2;
+      dst[at] = make_uint4(h[0], h[1], h[2], h[3]);
+      dst[at + 1] = make_uint4(h[4], h[5], h[6], h[7]);
+    }
+  } else {
+    const int nv = tiles * 16;
+    uint4* dst = reinterpret_cast<uint4*>(smem);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nv * rows; i += kBlock) {
+      const int r = i / nv, v = i - r * nv, k = k0 + v * 8;
+      uint4 q = make_uint4(0, 0, 0, 0);
+      const uint16_t* src = static_cast<const uint16_t*>(a.x) + (m0 + r) * a.ldx + k;
+      if (vec) {
+        if (k < a.K) q = __ldg(reinterpret_cast<const uint4*>(src));
+      } else {
+        uint32_t w[4] = {};
+        for (int e = 0; e < 8; e++)
+          if (k + e < a.K) w[e >> 1] |= (uint32_t)src[e] << (16 * (e & 1));
+        q = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      dst[((v >> 2) * rows + r) * 4 + (v & 3)] = q;
+    }
   }
-  for (int o = 16; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-  if (lane != 0) return;
-  if (a.x_scale) y *= a.x_scale[m];
-  if (a.bias) y += a.bias[n];
-  if (a.gelu) y = gelu_tanh(y);
-  if (a.out_dtype == SDQ_F32) store_dst<SDQ_F32>(a.out, i, y);
-  else if (a.out_dtype == SDQ_BF16) store_dst<SDQ_BF16>(a.out, i, y);
-  else store_dst<SDQ_F16>(a.out, i, y);
+}
+
+// XT, ST: types of the activations and of the scales.
+template <int XT, int ST, int GROUP>
+__global__ void __launch_bounds__(kBlock, kBlocksPerSm) w4_rows_kernel(const W4Args a, const W4Plan p, const int vec) {
+  constexpr bool BF = XT == SDQ_BF16;
+  constexpr int P = XT == SDQ_F32 ? 2 : 1;
+  constexpr int SS = ST == SDQ_F32 ? 4 : 2, kTile = kTileBytes(SS, GROUP), kScalePieces = (kTile - 1024) / 16;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float row_exp[kRows];   // fp32 rows: 2^e of the stage
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, c = lane & 3;
+  const int rank = blockIdx.x % p.ck, strip = blockIdx.x / p.ck;
+  // the first strips_long strips have p.strip row tiles, the others one less
+  const int strip_rows = strip < p.strips_long ? p.strip : p.strip - 1;
+  const int row0 = strip * p.strip - max(0, strip - p.strips_long);
+  const int m0 = blockIdx.y * kRows;
+  const int rows = (int)min((int64_t)kRows, a.M - m0);
+  const int k_tiles = (int)((a.K + 127) / 128);
+  const int slice0 = min(k_tiles, rank * p.slice), slice1 = min(k_tiles, slice0 + p.slice);
+  float* red = reinterpret_cast<float*>(smem + p.red);     // [warp][slot][row of x][16]
+  float* part = reinterpret_cast<float*>(smem + p.part);   // [row tile][row of x][16]
+  const int box = rows * 16;
+  const uint8_t* ring = smem + warp * (kAhead * kTile);
+  const uint32_t to_ring = (uint32_t)__cvta_generic_to_shared(ring);
+
+  allow_dependent_launch();
+  bool first = true;
+  for (int s0 = slice0; s0 < slice1 || first; s0 += p.stage) {   // once at least: a block without columns adds zeros
+    const int tiles = max(0, min(p.stage, slice1 - s0));
+    const int run = (strip_rows * tiles + kWarps - 1) / kWarps;
+    const int i0 = min(warp * run, strip_rows * tiles), i1 = min(i0 + run, strip_rows * tiles);
+    const int r0 = tiles > 0 ? i0 / tiles : 0, t0 = i0 - r0 * tiles;
+    // what the next fetch takes: tiles lie behind one another up to the end of the stage's row tile
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(a.q) + ((int64_t)(row0 + r0) * k_tiles + s0 + t0) * kTile + lane * 16;
+    const int64_t skip = (int64_t)(k_tiles - tiles) * kTile;
+    int to_end = tiles - t0, left = i1 - i0;
+    auto fetch = [&](uint32_t slot) {
+      if (left > 0) {
+        left--;
+        const uint32_t dst = to_ring + slot * kTile + lane * 16;
+        copy_async(dst, src);
+        copy_async(dst + 512, src + 512);
+        if (kScalePieces == 32 || lane < kScalePieces) copy_async(dst + 1024, src + 1024);
+        src += kTile;
+        if (--to_end == 0) {
+          src += skip;
+          to_end = tiles;
+        }
+      }
+      copies_commit();   // one group a tile, an empty one behind the last, so that their number tells which have landed
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) fetch(i);
+    if (first) wait_prior_grids();   // the weights are there from the upload on; x, bias and out belong to the stream
+    fill_x<XT>(a, m0, rows, s0 * 128, tiles, vec, smem + p.x, row_exp);
+    __syncthreads();
+    float ex[2] = {};
+    if constexpr (P == 2) {
+#pragma unroll
+      for (int j = 0; j < 2; j++) ex[j] = 2 * c + j < rows ? row_exp[2 * c + j] : 0.0f;
+    }
+    float y[4] = {}, acc[4];
+    // lanes of columns that no row of x fills read the last row: what they compute is never stored
+    const uint4* x_lane = reinterpret_cast<const uint4*>(smem + p.x) + min(g, rows - 1) * 4 + c;
+    const uint4* xb = x_lane + t0 * (4 * P * 4) * rows;
+    int to_store = tiles - t0, slot = 0;
+    uint32_t at = 0;
+    for (int i = i0; i < i1; i++) {
+      copies_wait<kAhead - 1>();
+      __syncwarp();   // the scales are other lanes' copies
+      const uint8_t* piece = ring + at * kTile;
+      const uint4 w0 = *reinterpret_cast<const uint4*>(piece + lane * 16), w1 = *reinterpret_cast<const uint4*>(piece + lane * 16 + 512);
+      const uint32_t words[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {      // 32 columns
+        uint4 b[P];
+#pragma unroll
+        for (int pl = 0; pl < P; pl++) b[pl] = xb[(j * P + pl) * 4 * rows];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          uint32_t af[4];
+          nibbles_to_16<BF>(words[2 * j + h], af);
+#pragma unroll
+          for (int pl = 0; pl < P; pl++) {
+            const uint2 bb = h == 0 ? make_uint2(b[pl].x, b[pl].y) : make_uint2(b[pl].z, b[pl].w);
+            if (pl == 0 && h == 0 && (32 * j) % GROUP % 64 == 0) mma16816<BF, true>(acc, af, bb);
+            else mma16816<BF, false>(acc, af, bb);
+          }
+        }
+        if ((32 * (j + 1)) % GROUP % 64 == 0) {   // at the end of a group, and after 64 columns of a long one
+          const float2 f = scale_pair<ST>(piece + 1024 + (32 * j / GROUP) * (16 * SS) + g * (2 * SS));
+          if constexpr (P == 2) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[e] *= ex[e & 1];
+          }
+          y[0] = fmaf(acc[0], f.x, y[0]);
+          y[1] = fmaf(acc[1], f.x, y[1]);
+          y[2] = fmaf(acc[2], f.y, y[2]);
+          y[3] = fmaf(acc[3], f.y, y[3]);
+        }
+      }
+      xb += (4 * P * 4) * rows;
+      __syncwarp();
+      fetch(at);   // the words of this slot are used up
+      at = at + 1 == kAhead ? 0 : at + 1;
+      if (--to_store == 0 || i + 1 == i1) {   // the row tile, or this warp's share of it, is done
+        float* dst = red + (warp * p.slots + slot) * box + g;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          if (2 * c + j < rows) {
+            dst[(2 * c + j) * 16] = y[j];
+            dst[(2 * c + j) * 16 + 8] = y[j + 2];
+          }
+        }
+        y[0] = y[1] = y[2] = y[3] = 0.0f;
+        to_store = tiles;
+        xb = x_lane;
+        slot++;
+      }
+    }
+    copies_wait<0>();
+    __syncthreads();
+    // ---- the block's sums: row tile r lies in the warps whose runs touch [r, r + 1) * tiles ----
+    for (int i = threadIdx.x; i < strip_rows * box; i += kBlock) {
+      const int r = i / box, e = i - r * box;
+      float s = first ? 0.0f : part[i];
+      if (tiles > 0) {
+        const int k0 = r * tiles / run, k1 = ((r + 1) * tiles - 1) / run;
+        for (int k = k0; k <= k1; k++) s += red[(k * p.slots + r - k * run / tiles) * box + e];
+      }
+      part[i] = s;
+    }
+    first = false;
+    if (s0 + p.stage < slice1) __syncthreads();   // x and the sums are read before the next stage writes them
+  }
+  auto finish = [&](int i, float s) {
+    const int r = i / box, m = (i - r * box) >> 4;
+    const int64_t n = ((int64_t)row0 + r) * 16 + (i & 15);
+    if (n >= a.N) return;
+    if (XT == SDQ_I8) s *= a.x_scale[m0 + m];
+    if (a.bias) s += a.bias[n];
+    if (a.gelu) s = gelu_tanh(s);
+    const int64_t o = (m0 + m) * a.N + n;
+    if (a.out_dtype == SDQ_F32) store_dst<SDQ_F32>(a.out, o, s);
+    else if (a.out_dtype == SDQ_BF16) store_dst<SDQ_BF16>(a.out, o, s);
+    else store_dst<SDQ_F16>(a.out, o, s);
+  };
+  const int count = strip_rows * box;
+  if (p.ck == 1) {
+    for (int i = threadIdx.x; i < count; i += kBlock) finish(i, part[i]);   // each thread its own sums
+  } else {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    for (int i = rank * kBlock + threadIdx.x; i < count; i += kBlock * p.ck) {
+      float s = 0.0f;
+      for (int r = 0; r < p.ck; r++) s += cluster.map_shared_rank(part, r)[i];
+      finish(i, s);
+    }
+    cluster.sync();   // nobody leaves while its sums may be read
+  }
+}
+
+constexpr int kSmemMost = 108 * 1024;   // of a block: two of them share an SM
+
+// The cut for clusters of ck blocks in `waves` rounds; false where shared memory does not hold even one
+// tile of x beside the rest.
+bool w4_cut(int64_t N, int64_t K, int rows, int planes, int ring, int ck, int waves, W4Plan* p, int* smem) {
+  const int clusters = ck == 1 ? 296 : ck == 2 ? 148 : ck == 4 ? 71 : 33;   // that run at a time, two blocks to an SM
+  const int n_tiles = (int)((N + 15) / 16), k_tiles = (int)((K + 127) / 128);
+  const int strips = (int)std::min<int64_t>(n_tiles, (int64_t)clusters * waves);
+  p->ck = ck;
+  p->strip = (n_tiles + strips - 1) / strips;
+  p->strips_long = n_tiles - strips * (p->strip - 1);
+  p->slice = (k_tiles + ck - 1) / ck;
+  const int tile_bytes = 128 * 2 * planes * rows;
+  for (int stages = 1; stages <= p->slice; stages++) {
+    p->stage = (p->slice + stages - 1) / stages;
+    // a run of ceil(strip * t / warps) pairs, t to a row tile, touches at most (run + t - 2) / t + 1 row
+    // tiles, which is no more than strip / warps + 2 for any t
+    p->slots = p->strip / kWarps + 2;
+    p->x = ring * kWarps;
+    p->red = p->x + p->stage * tile_bytes;
+    p->part = p->red + kWarps * p->slots * rows * 64;
+    *smem = p->part + p->strip * rows * 64;
+    if (*smem <= kSmemMost) return true;
+  }
+  return false;
+}
+
+// The cheapest of the four cluster sizes.  A larger cluster means a shorter slice of x to convert in every
+// block and a finer division of the row tiles, and costs a meeting of its blocks.  In clocks, measured:
+// 600 for a tile of a warp (1040 with fp32 rows, two products), 10 / 12 / 56 for 256 elements of x (16
+// bits / int8 / fp32), 0 / 900 / 1500 / 2000 for the meeting and 8 % for blocks that wait for each other.
+// One row, 4096 x 28672: 14.8 us without clusters, 16.0 / 17.0 / 19.2 with 2 / 4 / 8; 8 fp32 rows,
+// 14336 x 5003: 101 us without, 57 / 36 / 29 with.
+W4Plan w4_plan(const W4Args& a, int rows, int ring, int* smem) {
+  const int planes = a.x_dtype == SDQ_F32 ? 2 : 1;
+  W4Plan best{};
+  double least = 1e300;
+  for (int i = 0, ck = 1; i < 4; i++, ck *= 2) {
+    W4Plan p;
+    int bytes, waves = 1 + (int)(a.N / (16 * 160) * ck / 296);   // no strip of more than 160 tiles fits anyway
+    while (!w4_cut(a.N, a.K, rows, planes, ring, ck, waves, &p, &bytes)) waves++;
+    static const double kMeet[4] = {0, 900, 1500, 2000};
+    const double tiles = (p.strip * p.slice + kWarps - 1) / kWarps * (planes == 2 ? 1040.0 : 600.0);
+    const double fill = p.slice * 128.0 * rows / kBlock * (planes == 2 ? 56 : a.x_dtype == SDQ_I8 ? 12 : 10);
+    const double cost = waves * ((tiles + fill) * (ck > 1 ? 1.08 : 1.0) + kMeet[i]);
+    if (cost < least) { least = cost; best = p; *smem = bytes; }
+  }
+  return best;
+}
+
+template <int XT, int ST, int GROUP>
+cudaError_t launch_rows(const W4Args& a, cudaStream_t s) {
+  int smem = 0;
+  const W4Plan p = w4_plan(a, (int)std::min<int64_t>(a.M, kRows), kAhead * kTileBytes(ST == SDQ_F32 ? 4 : 2, GROUP), &smem);
+  static const cudaError_t set = cudaFuncSetAttribute(w4_rows_kernel<XT, ST, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+  if (set != cudaSuccess) return set;
+  const int n_tiles = (int)((a.N + 15) / 16);
+  const int strips = p.strips_long + (n_tiles - p.strips_long * p.strip) / std::max(1, p.strip - 1);
+  const int size = XT == SDQ_F32 ? 4 : XT == SDQ_I8 ? 1 : 2;
+  const int vec = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.ldx * size % 16 == 0 && a.K * size % 16 == 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(strips * p.ck), (unsigned)((a.M + kRows - 1) / kRows));
+  cfg.blockDim = dim3(kBlock);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim = {(unsigned)p.ck, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = p.ck > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, w4_rows_kernel<XT, ST, GROUP>, a, p, vec);
+}
+template <int XT, int ST>
+cudaError_t launch_group(const W4Args& a, cudaStream_t s) {
+  return a.group == 32 ? launch_rows<XT, ST, 32>(a, s) : a.group == 64 ? launch_rows<XT, ST, 64>(a, s) : launch_rows<XT, ST, 128>(a, s);
+}
+template <int XT>
+cudaError_t launch_scales(const W4Args& a, cudaStream_t s) {
+  return a.scale_dtype == SDQ_F32    ? launch_group<XT, SDQ_F32>(a, s)
+         : a.scale_dtype == SDQ_BF16 ? launch_group<XT, SDQ_BF16>(a, s) : launch_group<XT, SDQ_F16>(a, s);
 }
 
 template <int DT>
@@ -134,9 +568,8 @@ cudaError_t quantize_typed(const void* src, int64_t N, int64_t K, int group, uin
 
 }  // namespace
 
-size_t w4_bytes(int64_t N, int64_t K) { return (size_t)((N + 15) / 16) * (size_t)((K + 63) / 64) * 512; }
-size_t w4_scale_bytes(int64_t N, int64_t K, int group, int scale_dtype) {
-  return (size_t)((N + 15) / 16) * 16 * (size_t)((K + group - 1) / group) * (scale_dtype == SDQ_F32 ? 4 : 2);
+size_t w4_bytes(int64_t N, int64_t K, int group, int scale_dtype) {
+  return (size_t)((N + 15) / 16) * (size_t)((K + 127) / 128) * kTileBytes(scale_dtype == SDQ_F32 ? 4 : 2, group);
 }
 
 cudaError_t launch_w4_quantize(const void* src, int src_dtype, int64_t N, int64_t K, int group, uint8_t* q, void* scale,
@@ -150,19 +583,24 @@ cudaError_t launch_w4_quantize(const void* src, int src_dtype, int64_t N, int64_
 }
 
 cudaError_t launch_w4_layout(const uint8_t* q, const void* scale, int scale_dtype, int64_t N, int64_t K, int group,
-                             uint32_t* q_out, void* scale_out, cudaStream_t s) {
-  const int64_t words = (int64_t)(w4_bytes(N, K) / 4), groups = (K + group - 1) / group;
-  const int64_t scales = (N + 15) / 16 * 16 * groups;
-  count_launch(2);
-  w4_layout_kernel<<<148 * 8, kBlock, 0, s>>>(q, N, K, words, q_out);
-  if (scale_dtype == SDQ_F32) w4_scale_layout_kernel<4><<<148 * 2, kBlock, 0, s>>>(scale, N, groups, scales, scale_out);
-  else w4_scale_layout_kernel<2><<<148 * 2, kBlock, 0, s>>>(scale, N, groups, scales, scale_out);
+                             uint32_t* out, cudaStream_t s) {
+  const int64_t words = (int64_t)(w4_bytes(N, K, group, scale_dtype) / 4);
+  const int tile_words = kTileBytes(scale_dtype == SDQ_F32 ? 4 : 2, group) / 4;
+  const unsigned grid = (unsigned)std::min<int64_t>(148 * 16, (words + kBlock - 1) / kBlock);
+  count_launch();
+  if (scale_dtype == SDQ_F32) w4_layout_kernel<4><<<grid, kBlock, 0, s>>>(q, scale, N, K, group, tile_words, words, out);
+  else w4_layout_kernel<2><<<grid, kBlock, 0, s>>>(q, scale, N, K, group, tile_words, words, out);
   return cudaGetLastError();
 }
 
 cudaError_t launch_w4_matmul(const W4Args& a, cudaStream_t s) {
   count_launch();
-  return launch_overlapped(w4_simple_kernel, dim3((unsigned)((a.M * a.N + kBlock / 32 - 1) / (kBlock / 32))), dim3(kBlock), 0, s, a);
+  switch (a.x_dtype) {
+    case SDQ_F32: return launch_scales<SDQ_F32>(a, s);
+    case SDQ_BF16: return launch_scales<SDQ_BF16>(a, s);
+    case SDQ_F16: return launch_scales<SDQ_F16>(a, s);
+    default: return launch_scales<SDQ_I8>(a, s);
+  }
 }
 
 }  // namespace sdq
