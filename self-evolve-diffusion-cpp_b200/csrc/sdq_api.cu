@@ -884,9 +884,9 @@ static const char* kv_args(const sdq_kv_cache* c, const sdq_kv_seqs* s, int64_t 
   if (!c || !s) return "null descriptor";
   if (c->pages < 0 || c->heads <= 0 || c->page_size <= 0) return "bad cache shape";
   if (c->head_dim < 16 || c->head_dim > 128 || c->head_dim % 16 != 0) return "head_dim must be a multiple of 16 up to 128";
-  if (c->heads > (1 << 16) || c->page_size > (1 << 24) || c->pages > INT32_MAX / ((int64_t)c->heads * c->page_size))
+  if (c->heads > 65535 || c->page_size > (1 << 24) || c->pages > INT32_MAX / ((int64_t)c->heads * c->page_size))
     return "pages * heads * page_size must fit 31 bits";
-  if (s->batch < 0 || s->max_pages < 0 || (int64_t)s->max_pages * c->page_size > INT32_MAX) return "bad sequence table shape";
+  if (s->batch < 0 || s->batch > (1 << 24) || s->max_pages < 0 || (int64_t)s->max_pages * c->page_size > INT32_MAX) return "bad sequence table shape";
   if (rows < 0 || rows > INT32_MAX / 2) return "bad number of rows";
   if (c->pages > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale)) return "null pointer in the cache";
   if (s->batch > 0 && (!s->row_start || !s->kv_len || (s->max_pages > 0 && !s->page_table))) return "null pointer in the sequence table";
@@ -938,9 +938,9 @@ int sdq_kv_attention(const sdq_kv_cache* cache, const sdq_kv_seqs* seqs, const v
     if (const char* bad = kv_args(cache, seqs, rows, &a)) return invalid(kName, bad);
     if (!float_dtype(dtype)) return invalid(kName, "dtype must be SDQ_F32, SDQ_BF16 or SDQ_F16");
     if (flags & ~(uint32_t)(SDQ_SYNC | SDQ_CAUSAL)) return invalid(kName, "unsupported flag");
-    if (heads <= 0 || heads % a.heads != 0 || heads > (1 << 16)) return invalid(kName, "heads must be a positive multiple of the cache's heads");
+    if (heads <= 0 || heads % a.heads != 0 || heads > 65535) return invalid(kName, "heads must be a positive multiple of the cache's heads");
     if (!(scale > 0.0f) || scale > 1e30f) return invalid(kName, "scale must be positive and finite");
-    if (rows * (int64_t)heads > INT32_MAX) return invalid(kName, "rows * heads must fit 31 bits");
+    if (rows * (int64_t)heads > (1 << 30)) return invalid(kName, "rows * heads must fit 30 bits");
     const bool none = rows == 0 || a.batch == 0;
     if (!none && (!q_dev || !out_dev)) return invalid(kName, "null pointer");
     const int64_t width = (int64_t)heads * a.D;

@@ -109,7 +109,7 @@ def attention64(pool, q, heads, scale, causal, b):
     return out, mag, smag
 
 
-def attention_tolerance(name, keys, out, mag, smag):
+def attention_tolerance(name, pool, b, out, mag, smag):
     """What the kernel's roundings add up to at most, element by element.
 
     A score is off by its two factors' roundings (q in 11 bits of a power of two, or 22 with fp32; the
@@ -119,8 +119,15 @@ def attention_tolerance(name, keys, out, mag, smag):
     weight is rounded once more to 11 bits (16-bit types) or 22 (fp32), and the exponential is good to
     2^-21.  Sums over the keys are fp32: 2^-23 for each addition of 16 keys, both in the weights'
     sum and in the output.  Then the output's own rounding: half a step relative to the value, and for
-    fp16, whose numbers below 2^-14 lie on a grid of 2^-24, at least half of that grid (2^-25)."""
+    fp16, whose numbers below 2^-14 lie on a grid of 2^-24, at least half of that grid (2^-25).
+
+    Weights are fp16 numbers in units that put the largest v_scale of the sequence into [2^14, 2^15), and
+    fp16's grid ends at 2^-24: a weight is off by 2^-25 units, 2^-39 of that scale, however small it is.
+    Times codes of at most 2^7, for every key: keys * 2^-32 * max v_scale (the sum of the p is >= 1)."""
+    keys = pool.keys[b]
+    pg, off = pool.places(b)
+    vmax = float(pool.vs.cpu().numpy()[pg, :, off].max()) if keys else 0.0
     score = smag * (2.0 ** -22 + 16 * 2.0 ** -23 + 8 * 2.0 ** -24)
     weight = 2.0 ** -11 if name != "f32" else 2.0 ** -21
     rel = 2 * score + weight + 2.0 ** -20 + 2 * (keys / 16 + 8) * 2.0 ** -23
-    return rel[..., None] * mag + half_step(name) * np.abs(out) + (2.0 ** -25 if name == "f16" else 1e-30)
+    return rel[..., None] * mag + half_step(name) * np.abs(out) + (2.0 ** -25 if name == "f16" else 1e-30) + keys * 2.0 ** -32 * vmax

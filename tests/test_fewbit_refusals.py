@@ -97,7 +97,7 @@ def seqs(pkg, **kw):
     (dict(pages=1 << 40), {}, "31 bits"), (dict(pages=1 << 30, heads=1, page_size=2), {}, "31 bits"),
     (dict(k=None), {}, "null pointer in the cache"), (dict(v_scale=None), {}, "null pointer in the cache"),
     (dict(k=P + 8), {}, "16-byte"), (dict(v_scale=P + 2), {}, "aligned"),
-    ({}, dict(batch=-1), "sequence table shape"), ({}, dict(max_pages=-1), "sequence table shape"),
+    ({}, dict(batch=-1), "sequence table shape"), ({}, dict(batch=1 << 25), "sequence table shape"), ({}, dict(max_pages=-1), "sequence table shape"),
     ({}, dict(max_pages=1 << 30), "sequence table shape"), ({}, dict(row_start=None), "null pointer in the sequence"),
     ({}, dict(kv_len=None), "null pointer in the sequence"), ({}, dict(page_table=None), "null pointer in the sequence"),
     ({}, dict(kv_len=P + 1), "aligned"),
@@ -128,7 +128,7 @@ def test_kv_calls(lib, pkg):
     refused(lib, a(c, s, P, 0, 0, 4, 2, 0.0, P, 0, 0, None), "scale")
     refused(lib, a(c, s, P, 0, 0, 4, 2, float("nan"), P, 0, 0, None), "scale")
     refused(lib, a(c, s, P, 0, 0, 4, 2, float("inf"), P, 0, 0, None), "scale")
-    refused(lib, a(c, s, P, 0, 0, 1 << 29, 8, 0.1, P, 0, 0, None), "31 bits")
+    refused(lib, a(c, s, P, 0, 0, 1 << 29, 8, 0.1, P, 0, 0, None), "30 bits")
     refused(lib, a(c, s, None, 0, 0, 4, 2, 0.1, P, 0, 0, None), "null pointer")
     refused(lib, a(c, s, P, 0, 100, 4, 2, 0.1, P, 0, 0, None), "stride")
     refused(lib, a(c, s, P, 0, 0, 4, 2, 0.1, P, 100, 0, None), "stride")

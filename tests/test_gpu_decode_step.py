@@ -87,7 +87,7 @@ class Layer:
                 stored = pool.dense(i, which)[pool.keys[i] - n:]
                 assert np.array_equal(stored, codes.astype(np.float64) * sc[..., None].astype(np.float64))
             want, mag, smag = attention64(pool, c["q"].double().numpy(), HEADS, HD ** -0.5, True, i)
-            tol = attention_tolerance(name, pool.keys[i], want, mag, smag)
+            tol = attention_tolerance(name, pool, i, want, mag, smag)
             assert (np.abs(c["att"][first:first + n].double().numpy() - want) <= tol).all()
         linear("o", c["att"], None, c["o"])
         norm(1, c["o"], c["x"], c["sum1"])

@@ -137,7 +137,7 @@ def compare(pool, out, q, heads, name, scale, causal):
         want, mag, smag = attention64(pool, q64, heads, scale, causal, b)
         rows = slice(int(pool.starts[b]), int(pool.starts[b]) + pool.new[b])
         covered[rows] = True
-        tol = attention_tolerance(name, pool.keys[b], want, mag, smag)
+        tol = attention_tolerance(name, pool, b, want, mag, smag)
         err = np.abs(got[rows] - want)
         assert (err <= tol).all(), (b, np.nanmax(err / tol), np.isnan(err).sum())
     assert (got[~covered] == 11.0).all()      # rows of no sequence are left alone
