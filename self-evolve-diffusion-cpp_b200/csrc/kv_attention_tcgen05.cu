@@ -1,0 +1,613 @@
+// Attention of many new rows over the paged int8 cache, on tcgen05.
+//
+// One CTA per (128 rows, cache head); a row is a (token, query head) pair, so the heads that share a
+// cache head fill one tile together.  14 warps:
+//   warps 0..7   : softmax, one thread per row and half of a block's 128 keys (two threads share a row)
+//   warps 8..11  : converters: the cache's int8 pages -> fp16 operand tiles in shared memory
+//   warp 12      : MMA issuer of the scores, S = Q K^T, Q as A operand in tensor memory
+//   warp 13      : MMA issuer of O += P V, P in tensor memory (written in place over S)
+// Tensor memory (512 columns): Q hi 0..63, Q lo 64..127, O 128..255, S / P buffers 256..383, 384..511.
+//
+// The cached integers are exact in fp16, so a product takes one MMA for each fp16 number that the other
+// factor is made of: one for bf16 and fp16 queries, two (hi + lo, 22 bits) for fp32 ones.  The keys' scales
+// enter with the scores and the values' with the weights, w = p * v_scale / 2^ev, where 2^ev bounds the
+// sequence's v scales (found in a pass over them: 4 of the 2 (D + 4) bytes of a key).
+//
+// Softmax in one sweep with a running offset m of each row: p = 2^10 2^(s - m); the offset moves, and O and
+// the row's sum are scaled down, only when a block's maximum exceeds it by more than 4 log2 units, so a
+// weight stays below 2^14 and inside fp16.  The two threads of a row agree on a block's maximum through
+// shared memory.  With fp32 queries O is taken out of tensor memory every kDrain blocks and added up in
+// shared memory in fp32: the tensor core's accumulator truncates, and over thousands of keys that would be
+// the largest error there is (1e-5 of the result at 4k keys).
+//
+// Bound by: the softmax (a block's 128 x 128 weights take 1024 cycles of the exponential unit and ~1200 of
+// issue) with the conversion beside it (~450); the MMAs need 512..1024 per product.
+//
+// Every mbarrier wait is bounded like the GEMM kernels'.
+#include "kv_common.cuh"
+#include "tc_common.cuh"
+
+namespace sdq {
+namespace {
+using namespace tc;
+
+constexpr int kRowsT = 128;        // rows of a tile
+constexpr int kKeys = 128;         // keys of a block
+constexpr int kPlane = kKeys * 128 * 2;        // 32 KiB: a block's keys or values in fp16
+constexpr int kThreadsT = 448;
+constexpr int kDrain = 4;          // blocks between two drains of O (fp32 queries)
+constexpr uint32_t kColQhi = 0, kColQlo = 64, kColO = 128, kColS = 256;
+constexpr float kShift = 10.0f;    // weights are 2^10 times p
+constexpr float kStepUp = 4.0f;    // log2 units by which a block's maximum may exceed the running offset
+
+// Shared memory behind the operand tiles.
+struct Book {
+  float ks[4][kKeys], vs[4][kKeys];   // scales of the blocks under way
+  uint32_t there[4][4];               // which of their keys exist
+  int rows[4][kKeys];                 // pool rows
+  float meet[2][2][kRowsT];           // what the two threads of a row tell each other
+  float sum[2][kRowsT];
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pready[2], pvdone[2], scales[4], qready, lready, ofull, pair[4];
+  uint32_t v_top;
+  uint32_t tmem;
+  int abort;
+};
+constexpr int kSlack = 1024;       // to bring the dynamic base to a 1024-byte boundary
+template <int P>
+constexpr int kSmemMany = 4 * kPlane + (P == 2 ? 128 * kRowsT * 4 : 0) + (int)sizeof(Book) + kSlack;
+
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t rest_bits(uint32_t hi, float x, float y) {   // fp16 of what `hi` leaves of x and y
+  const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return half2_bits(x - back.x, y - back.y);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, const AttendArgs t, const int vec_q, const int vec_out) {
+  constexpr int P = DT == SDQ_F32 ? 2 : 1;
+  constexpr int EPV = Vec<DT>::EPV;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  const uint32_t smem_v = base + 2 * kPlane;
+  float* drained = reinterpret_cast<float*>(smem + 4 * kPlane);   // [d][row], fp32 queries
+  Book& bk = *reinterpret_cast<Book*>(smem + 4 * kPlane + (P == 2 ? 128 * kRowsT * 4 : 0));
+  volatile int* abort_flag = &bk.abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kh = blockIdx.y, group = t.heads / a.heads;
+
+  wait_prior_grids();
+  Tile tile;
+  // the last tiles of a causal sequence see the most keys: they go first
+  if (!find_tile(a, group, kRowsT, (int)(gridDim.x - 1 - blockIdx.x), &tile)) return;
+  const int last_token = (tile.first_row + tile.rows - 1) / group;
+  const int last_pos = t.causal ? (int)max((int64_t)-1, (int64_t)table_at(a.kv_len, tile.b) - tile.n + last_token) : INT_MAX;
+  const int keys = max(0, t.causal ? (last_pos < tile.len ? last_pos + 1 : tile.len) : tile.len);
+  const int nblk = (keys + kKeys - 1) / kKeys;
+  auto place = [&](int p) {   // pool row of key p for this cache head, -1: absent
+    const int r = p < keys ? pool_row(a, tile.b, p) : -1;
+    return r < 0 ? -1 : r + kh * a.page_size;
+  };
+  auto bar = [&](const uint64_t& b) { return smem_u32(&b); };
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; i++) {
+      mbar_init(bar(bk.kfull[i]), 4);
+      mbar_init(bar(bk.kempty[i]), 1);
+      mbar_init(bar(bk.vfull[i]), 4);
+      mbar_init(bar(bk.vempty[i]), 1);
+      mbar_init(bar(bk.sfull[i]), 1);
+      mbar_init(bar(bk.pready[i]), 8);
+      mbar_init(bar(bk.pvdone[i]), 1);
+    }
+    for (int i = 0; i < 4; i++) {
+      mbar_init(bar(bk.scales[i]), 4);
+      mbar_init(bar(bk.pair[i]), 2);
+    }
+    mbar_init(bar(bk.qready), 8);
+    mbar_init(bar(bk.lready), 8);
+    mbar_init(bar(bk.ofull), 1);
+    bk.abort = 0;
+    bk.v_top = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 12) {
+    tmem_alloc(smem_u32(&bk.tmem), 512);
+    tmem_relinquish();
+  }
+  // the largest v scale of the keys
+  {
+    float top = 0.0f;
+    for (int p0 = threadIdx.x; p0 < keys; p0 += 8 * kThreadsT) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int r = place(p0 + i * kThreadsT);
+        x[i] = r >= 0 ? fabsf(__ldg(a.v_scale + r)) : 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) top = fmaxf(top, x[i]);
+    }
+    top = warp_max(top);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (lane == 0) atomicMax(&bk.v_top, __float_as_uint(top));   // positive floats order as integers
+    __syncthreads();
+  }
+  const uint32_t tmem_base = bk.tmem;
+  const int ev = min(max((int)(bk.v_top >> 23) - 126, -126), 126);   // v_scale < 2^ev (where it is finite)
+
+  if (warp >= 8 && warp < 12) {
+    // ---------------------------------------------------------------- converters
+    const int w = warp - 8, tt = threadIdx.x - 256;       // 0..127
+    const int piece = tt & 7, krow = tt >> 3;             // keys: 16 bytes of d, key krow + 16 i
+    const int dw = lane & 7, kg = lane >> 3;              // values: 4 of this warp's 32 values of d, 8 of 32 keys
+    const bool has_k = piece * 16 < a.D, has_v = 32 * w + 4 * dw < a.D;
+    const float unit = pow2f(-ev);
+    auto key_of = [&](int j) { return j < nblk ? place(j * kKeys + tt) : -1; };
+    uint4 kr[8];
+    uint32_t vr[4][8];
+    auto load_k = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int row = bk.rows[j & 3][krow + 16 * i];
+        kr[i] = make_uint4(0, 0, 0, 0);
+        if (row >= 0 && has_k) kr[i] = __ldg(reinterpret_cast<const uint4*>(a.k + (int64_t)row * a.D + piece * 16));
+      }
+    };
+    auto load_v = [&](int j) {
+#pragma unroll
+      for (int it = 0; it < 4; it++) {
+        const int4* rp = reinterpret_cast<const int4*>(&bk.rows[j & 3][it * 32 + kg * 8]);
+        const int4 r0 = rp[0], r1 = rp[1];
+        const int rows[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          vr[it][e] = 0;
+          if (rows[e] >= 0 && has_v) vr[it][e] = __ldg(reinterpret_cast<const uint32_t*>(a.v + (int64_t)rows[e] * a.D + 32 * w + 4 * dw));
+        }
+      }
+    };
+    int row_now = key_of(0), row_next = key_of(1);
+    bk.rows[0][tt] = row_now;
+    bk.rows[1][tt] = row_next;
+    float ks = row_now >= 0 ? __ldg(a.k_scale + row_now) : 0.0f, vs = row_now >= 0 ? __ldg(a.v_scale + row_now) : 0.0f;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (nblk > 0) {
+      load_k(0);
+      load_v(0);
+    }
+    bool ok = true;   // after a wait that gave up the loop only keeps the warps' meetings
+    for (int j = 0; j < nblk; j++) {
+      const int row_2 = key_of(j + 2);
+      const uint32_t slot = j & 1, ph = (j >> 1) & 1;
+      ok = ok && mbar_wait_warp(bar(bk.kempty[slot]), ph ^ 1u, abort_flag, t.status, 0xc00 | 1);
+      if (ok) {
+        const uint32_t st = base + slot * kPlane + (piece >> 2) * 16384;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const uint32_t x[4] = {kr[i].x ^ 0x80808080u, kr[i].y ^ 0x80808080u, kr[i].z ^ 0x80808080u, kr[i].w ^ 0x80808080u};
+          uint32_t h[8];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            h[2 * e] = bytes_to_half2(x[e], 0x4140);
+            h[2 * e + 1] = bytes_to_half2(x[e], 0x4342);
+          }
+          const int key = krow + 16 * i, c0 = 2 * (piece & 3);
+          const uint32_t row = st + key * 128;
+          // the second 64 values of d store their odd chunk first: the two halves use other banks
+          if (piece < 4) {
+            st_shared_v4_b32(row + ((c0 ^ (key & 7)) << 4), h[0], h[1], h[2], h[3]);
+            st_shared_v4_b32(row + (((c0 + 1) ^ (key & 7)) << 4), h[4], h[5], h[6], h[7]);
+          } else {
+            st_shared_v4_b32(row + (((c0 + 1) ^ (key & 7)) << 4), h[4], h[5], h[6], h[7]);
+            st_shared_v4_b32(row + ((c0 ^ (key & 7)) << 4), h[0], h[1], h[2], h[3]);
+          }
+        }
+        bk.ks[j & 3][tt] = ks;
+        bk.vs[j & 3][tt] = vs * unit;
+        const uint32_t there = __ballot_sync(0xffffffffu, row_now >= 0);
+        if (lane == 0) bk.there[j & 3][w] = there;
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bar(bk.kfull[slot]));
+          mbar_arrive(bar(bk.scales[j & 3]));
+        }
+        if (j + 1 < nblk) load_k(j + 1);
+      }
+      ok = ok && mbar_wait_warp(bar(bk.vempty[slot]), ph ^ 1u, abort_flag, t.status, 0xc00 | 2);
+      if (ok) {
+        if (32 * w < a.D) {
+#pragma unroll
+          for (int it = 0; it < 4; it++) {
+            uint32_t h[4][4];   // [value of d][pair of keys]
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              const uint32_t x = __byte_perm(vr[it][e], vr[it][e + 1], 0x5140) ^ 0x80808080u;
+              const uint32_t y = __byte_perm(vr[it][e], vr[it][e + 1], 0x7362) ^ 0x80808080u;
+              h[0][e / 2] = bytes_to_half2(x, 0x4140);
+              h[1][e / 2] = bytes_to_half2(x, 0x4342);
+              h[2][e / 2] = bytes_to_half2(y, 0x4140);
+              h[3][e / 2] = bytes_to_half2(y, 0x4342);
+            }
+            const int chunk = (it & 1) * 4 + kg;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const int d = 32 * w + 4 * dw + i;
+              st_shared_v4_b32(smem_v + slot * kPlane + (it >> 1) * 16384 + d * 128 + ((chunk ^ (d & 7)) << 4), h[i][0], h[i][1], h[i][2], h[i][3]);
+            }
+          }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(bk.vfull[slot]));
+        if (j + 1 < nblk) load_v(j + 1);
+      }
+      row_now = row_next;
+      row_next = row_2;
+      bk.rows[(j + 2) & 3][tt] = row_2;
+      ks = row_now >= 0 ? __ldg(a.k_scale + row_now) : 0.0f;
+      vs = row_now >= 0 ? __ldg(a.v_scale + row_now) : 0.0f;
+      asm volatile("bar.sync 1, 128;" ::: "memory");   // the next rows are there
+    }
+  } else if (warp == 12) {
+    if (lane == 0 && nblk > 0) {
+      // -------------------------------------------------------------- scores
+      constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kRowsT >> 4) << 24);
+      bool ok = mbar_wait_spin(bar(bk.qready), 0, abort_flag, t.status, 0xc00 | 3);
+      for (int j = 0; ok && j < nblk; j++) {
+        const uint32_t slot = j & 1, ph = (j >> 1) & 1;
+        ok = mbar_wait_spin(bar(bk.kfull[slot]), ph, abort_flag, t.status, 0xc00 | 4);
+        if (ok && j >= 2) ok = mbar_wait_spin(bar(bk.pvdone[slot]), ph ^ 1u, abort_flag, t.status, 0xc00 | 5);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + kColS + slot * kKeys, st = base + slot * kPlane;
+        for (int ks = 0; ks < a.D / 16; ks++) {
+          const uint64_t k = make_smem_desc(st + (ks >> 2) * 16384) + (uint64_t)((ks & 3) * 2);
+          if constexpr (P == 2) umma_f16_ts(d, tmem_base + kColQlo + ks * 8, k, kIdesc, ks != 0);
+          umma_f16_ts(d, tmem_base + kColQhi + ks * 8, k, kIdesc, P == 2 || ks != 0);
+        }
+        umma_commit(bar(bk.kempty[slot]));
+        umma_commit(bar(bk.sfull[slot]));
+      }
+    }
+  } else if (warp == 13) {
+    if (lane == 0 && nblk > 0) {
+      // -------------------------------------------------------------- P V
+      const uint32_t idesc = (1u << 4) | ((uint32_t)(a.D >> 3) << 17) | ((uint32_t)(kRowsT >> 4) << 24);
+      bool ok = true;
+      for (int j = 0; ok && j < nblk; j++) {
+        const uint32_t slot = j & 1, ph = (j >> 1) & 1;
+        ok = mbar_wait_spin(bar(bk.pready[slot]), ph, abort_flag, t.status, 0xc00 | 6);
+        if (ok) ok = mbar_wait_spin(bar(bk.vfull[slot]), ph, abort_flag, t.status, 0xc00 | 7);
+        if (!ok) break;
+        tc_fence_after();
+        const bool fresh = P == 2 ? j % kDrain == 0 : j == 0;   // O was taken out (or is new)
+        const uint32_t p0 = tmem_base + kColS + slot * kKeys;
+#pragma unroll
+        for (int ks = 0; ks < kKeys / 16; ks++) {
+          const uint64_t v = make_smem_desc(smem_v + slot * kPlane + (ks >> 2) * 16384) + (uint64_t)((ks & 3) * 2);
+          // the weights of keys 32 c + 16 i .. lie in 8 columns: hi at 32 c + 8 i, lo 16 further
+          const uint32_t p = p0 + (ks >> 1) * 32 + (ks & 1) * 8;
+          if constexpr (P == 2) umma_f16_ts(tmem_base + kColO, p + 16, v, idesc, !(fresh && ks == 0));
+          umma_f16_ts(tmem_base + kColO, p, v, idesc, P == 2 || !(fresh && ks == 0));
+        }
+        umma_commit(bar(bk.vempty[slot]));
+        umma_commit(bar(bk.pvdone[slot]));
+      }
+      if (ok) umma_commit(bar(bk.ofull));
+    }
+  } else if (warp < 8) {
+    // ---------------------------------------------------------------- softmax
+    const int quarter = warp & 3, grp = warp >> 2, r = quarter * 32 + lane;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const int rr = tile.first_row + r, token = rr / group, head = kh * group + (rr - token * group);
+    const bool live = r < tile.rows;
+    const int seen = !live ? 0 : t.causal ? max(0, last_pos - last_token + token + 1) : INT_MAX;   // keys in front of the row's end
+    uint32_t pair_ph = 0;
+    bool ok = true;
+    auto pair_sync = [&]() {   // this warp and the one with the other half of the same rows
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(bk.pair[quarter]));
+      const bool done = mbar_wait_warp(bar(bk.pair[quarter]), pair_ph, abort_flag, t.status, 0xc00 | 8);
+      pair_ph ^= 1u;
+      return done;
+    };
+    // ---- q: this thread's half of the row, 64 values of d ----
+    float factor;
+    {
+      float q[64];
+      float mx = 0.0f;
+      const int64_t at = (int64_t)(tile.first + token) * t.ldq + (int64_t)head * a.D + grp * 64;
+#pragma unroll
+      for (int i = 0; i < 64; i += 8) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) q[i + e] = 0.0f;
+        if (live && grp * 64 + i < a.D) {
+          if (vec_q) {
+#pragma unroll
+            for (int e = 0; e < 8; e += EPV) {
+              float y[EPV];
+              Vec<DT>::unpack(__ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(t.q) + (at + i + e) * (16 / EPV))), y);
+#pragma unroll
+              for (int f = 0; f < EPV; f++) q[i + e + f] = y[f];
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) q[i + e] = load_src<DT>(t.q, at + i + e);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) mx = fold_abs(mx, q[i + e]);
+      }
+      bk.meet[0][grp][r] = mx;
+      ok = pair_sync();
+      mx = fmaxf(mx, bk.meet[0][grp ^ 1][r]);
+      // largest |q| of the row into [2^14, 2^15); a row with an infinity has no softmax: all NaN
+      const bool finite = mx <= 3.402823466e38f;
+      const int e = mx > 0.0f && finite ? max(ilogbf(mx) - 14, -126) : 0;
+      const float inv = finite ? pow2f(-e) : __uint_as_float(0x7fc00000u);
+      factor = fmaxf(pow2f(e) * t.scale * kLog2e, 1.17549435e-38f);   // not zero: -inf times it has to stay -inf
+      uint32_t hi[32];
+#pragma unroll
+      for (int i = 0; i < 32; i++) hi[i] = half2_bits(q[2 * i] * inv, q[2 * i + 1] * inv);
+      tmem_st_32x32(tmem_base + kColQhi + grp * 32 + lane_base, hi);
+      if constexpr (P == 2) {
+        uint32_t lo[32];
+#pragma unroll
+        for (int i = 0; i < 32; i++) lo[i] = rest_bits(hi[i], q[2 * i] * inv, q[2 * i + 1] * inv);
+        tmem_st_32x32(tmem_base + kColQlo + grp * 32 + lane_base, lo);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(bk.qready));
+    }
+    float m = -INFINITY, e_off = 0.0f, l = 0.0f;
+    for (int j = 0; ok && j < nblk; j++) {
+      const uint32_t slot = j & 1, ph = (j >> 1) & 1;
+      ok = mbar_wait_warp(bar(bk.scales[j & 3]), (j >> 2) & 1, abort_flag, t.status, 0xc00 | 9);
+      if (ok) ok = mbar_wait_warp(bar(bk.sfull[slot]), ph, abort_flag, t.status, 0xc00 | 10);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t s_col = tmem_base + kColS + slot * kKeys + grp * 64 + lane_base;
+      uint32_t s[2][32];
+      tmem_ld_32x32(s_col, s[0]);
+      tmem_ld_32x32(s_col + 32, s[1]);
+      tmem_ld_wait();
+      const float4* ks = reinterpret_cast<const float4*>(&bk.ks[j & 3][grp * 64]);
+      const float4* vs = reinterpret_cast<const float4*>(&bk.vs[j & 3][grp * 64]);
+      const int left = seen - (j * kKeys + grp * 64);   // keys of this half that the row sees
+      uint32_t sees[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+        sees[h] = bk.there[j & 3][grp * 2 + h] & (left >= 32 * h + 32 ? 0xffffffffu : left <= 32 * h ? 0u : (1u << (left - 32 * h)) - 1);
+      const bool all = __all_sync(0xffffffffu, (sees[0] & sees[1]) == 0xffffffffu);
+      float bm = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 k4 = ks[h * 8 + i / 4];
+          const float kk[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[h][i + e] = __float_as_uint(__uint_as_float(s[h][i + e]) * kk[e]);
+        }
+        if (!all) {
+#pragma unroll
+          for (int i = 0; i < 32; i++)
+            if (!((sees[h] >> i) & 1)) s[h][i] = 0xff800000u;   // -inf
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i++) bm = fmaxf(bm, __uint_as_float(s[h][i]));
+      }
+      bk.meet[j & 1][grp][r] = bm;    // alternating, so that one meeting a block is enough
+      ok = pair_sync();
+      if (!ok) break;
+      bm = fmaxf(bm, bk.meet[j & 1][grp ^ 1][r]);
+      const bool grow = (bm - m) * factor > kStepUp;   // true in the row's first block with a key
+      const bool drain = P == 2 && j > 0 && j % kDrain == 0;
+      const bool any = __any_sync(0xffffffffu, grow);
+      if (any || drain) {
+        float f = 1.0f;
+        if (grow) {
+          f = exp2_fast((m - bm) * factor);
+          m = bm;
+          e_off = kShift - m * factor;
+          l *= f;
+        }
+        if (j > 0) {
+          // O holds the blocks so far: the last P V must be done before O is scaled or taken out (the
+          // next one waits for this block's weights)
+          ok = mbar_wait_warp(bar(bk.pvdone[(j - 1) & 1]), ((j - 1) >> 1) & 1, abort_flag, t.status, 0xc00 | 11);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 2 * grp; c < 2 * grp + 2; c++) {
+            if (c * 32 >= a.D) break;
+            uint32_t o[32];
+            tmem_ld_32x32(tmem_base + kColO + c * 32 + lane_base, o);
+            tmem_ld_wait();
+            if constexpr (P == 2) {
+              float* d = drained + c * 32 * kRowsT + r;
+              if (drain) {
+#pragma unroll
+                for (int i = 0; i < 32; i++) d[i * kRowsT] = j == kDrain ? __uint_as_float(o[i]) * f : (d[i * kRowsT] + __uint_as_float(o[i])) * f;
+                continue;
+              }
+              if (j >= kDrain) {
+#pragma unroll
+                for (int i = 0; i < 32; i++) d[i * kRowsT] *= f;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st_32x32(tmem_base + kColO + c * 32 + lane_base, o);
+          }
+        }
+      }
+      float lb[2] = {};   // the block's sum by itself: fewer roundings than one long chain
+      // each 32 columns of scores become 16 of fp16 pairs of weights (hi), then 16 of what is left (lo)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        uint32_t hi[32];
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 v4 = vs[h * 8 + i / 4];
+          const float vv[4] = {v4.x, v4.y, v4.z, v4.w};
+          float wt[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float p = exp2_fast(fmaf(__uint_as_float(s[h][i + e]), factor, e_off));
+            lb[e & 1] += p;
+            wt[e] = p * vv[e];
+          }
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            const uint32_t x = half2_bits(wt[e], wt[e + 1]);
+            hi[(i + e) / 2] = x;
+            if constexpr (P == 2) hi[16 + (i + e) / 2] = rest_bits(x, wt[e], wt[e + 1]);
+          }
+        }
+        if constexpr (P == 2) {
+          tmem_st_32x32(s_col + 32 * h, hi);
+        } else {
+          uint32_t h16[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) h16[i] = hi[i];
+          tmem_st_32x16(s_col + 32 * h, h16);
+        }
+      }
+      l += lb[0] + lb[1];
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(bk.pready[slot]));
+    }
+    // ---- both halves' sums, then O / l ----
+    if (ok) {
+      bk.sum[grp][r] = l;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(bk.lready));
+      ok = mbar_wait_warp(bar(bk.lready), 0, abort_flag, t.status, 0xc00 | 12);
+    }
+    if (ok && nblk > 0) ok = mbar_wait_warp(bar(bk.ofull), 0, abort_flag, t.status, 0xc00 | 13);
+    if (ok) {
+      tc_fence_after();
+      l = bk.sum[0][r] + bk.sum[1][r];
+      const float inv = l != 0.0f ? (1.0f / l) * pow2f(ev) : 0.0f;   // a row that sees no key is zero
+      const int64_t at = (int64_t)(tile.first + token) * t.ldo + (int64_t)head * a.D;
+#pragma unroll 1
+      for (int c = 2 * grp; c < 2 * grp + 2; c++) {
+        if (c * 32 >= a.D) break;
+        float o[32];
+        if (nblk > 0) {
+          uint32_t x[32];
+          tmem_ld_32x32(tmem_base + kColO + c * 32 + lane_base, x);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; i++) {
+            o[i] = __uint_as_float(x[i]);
+            if constexpr (P == 2) {
+              if (nblk > kDrain) o[i] += drained[(c * 32 + i) * kRowsT + r];
+            }
+            o[i] = l != 0.0f ? o[i] * inv : 0.0f;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i++) o[i] = 0.0f;
+        }
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 32; i += EPV) {
+            if (c * 32 + i >= a.D) break;
+            float y[EPV];
+#pragma unroll
+            for (int e = 0; e < EPV; e++) y[e] = o[i + e];
+            if (vec_out) {
+              *reinterpret_cast<uint4*>(static_cast<char*>(t.out) + (at + c * 32 + i) * (16 / EPV)) = Vec<DT>::pack(y);
+            } else {
+#pragma unroll
+              for (int e = 0; e < EPV; e++) store_dst<DT>(t.out, at + c * 32 + i + e, y[e]);
+            }
+          }
+        }
+      }
+      tc_fence_before();
+    }
+  }
+
+  // -------------------------------------------------------------------- common exit
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (*abort_flag) {
+    for (int i = 0; i < 1000; i++) __nanosleep(1000);   // let MMAs in flight end (~1 ms)
+    __syncthreads();
+  }
+  if (warp == 12) {
+    __syncwarp();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+template <int DT>
+cudaError_t launch_typed(const KvArgs& a, const AttendArgs& t, cudaStream_t s) {
+  constexpr int P = DT == SDQ_F32 ? 2 : 1, size = DT == SDQ_F32 ? 4 : 2;
+  const int group = t.heads / a.heads;
+  const int64_t tiles = (int64_t)a.rows * group / kRowsT + a.batch;
+  const int vec_q = (reinterpret_cast<uintptr_t>(t.q) & 15) == 0 && t.ldq * size % 16 == 0;
+  const int vec_out = (reinterpret_cast<uintptr_t>(t.out) & 15) == 0 && t.ldo * size % 16 == 0;
+  return launch_overlapped(kv_attend_many<DT>, dim3((unsigned)tiles, (unsigned)a.heads), dim3(kThreadsT), kSmemMany<P>, s, a, t, vec_q, vec_out);
+}
+
+}  // namespace
+
+int kv_attend_many_setup(std::string* why) {
+  cudaError_t e = cudaFuncSetAttribute(kv_attend_many<SDQ_F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMany<2>);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kv_attend_many<SDQ_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMany<1>);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kv_attend_many<SDQ_F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMany<1>);
+  if (e != cudaSuccess) {
+    if (why) *why = std::string("cache attention set-up: ") + cudaGetErrorString(e);
+    return SDQ_ERR_CUDA;
+  }
+  return SDQ_OK;
+}
+
+cudaError_t launch_kv_attend_many(const KvArgs& a, const AttendArgs& t, int dtype, cudaStream_t s) {
+  if (dtype == SDQ_F32) return launch_typed<SDQ_F32>(a, t, s);
+  if (dtype == SDQ_BF16) return launch_typed<SDQ_BF16>(a, t, s);
+  return launch_typed<SDQ_F16>(a, t, s);
+}
+
+}  // namespace sdq

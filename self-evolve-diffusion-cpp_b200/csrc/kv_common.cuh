@@ -47,6 +47,7 @@ struct AttendArgs {
   int32_t heads;    // query heads, a multiple of the cache's
   int32_t causal;
   float scale;
+  int* status;      // device word for a wait that gave up
 };
 
 // Row range of sequence b, whatever the table holds: [first, last) inside [0, rows].
@@ -89,7 +90,66 @@ __host__ __device__ __forceinline__ int pool_row_of(const KvArgs& a, int row) {
   return p > INT32_MAX ? -1 : p < 0 ? -1 : pool_row(a, b, (int)p);
 }
 
+// Row tiles.  The rows of a sequence and one cache head are its new tokens times the `group` query heads
+// that share the head, row = token * group + head; a tile takes T of them.  The tiles of all sequences
+// are numbered without a table: sequence b's begin at row_start[b] * group / T + b, which leaves room for
+// a ragged last one (ceil(n / T) <= floor((s + n) / T) - floor(s / T) + 1); a number that is no tile ends
+// at once.
+struct Tile {
+  int b, first_row, rows;   // sequence; first (token, head) row; how many
+  int first, n, len;        // first row of the call, new tokens, keys of the sequence
+};
+__device__ __forceinline__ bool find_tile(const KvArgs& a, int group, int T, int id, Tile* t) {
+  // the last b whose tiles begin at or before id: their first numbers do not decrease, 32 at a time
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    bool at_or_before = false;
+    if (b0 + lane < a.batch) {
+      int f, l;
+      seq_rows(a, b0 + lane, f, l);
+      at_or_before = (int64_t)f * group / T + b0 + lane <= id;
+    }
+    const uint32_t all = __ballot_sync(0xffffffffu, at_or_before);
+    before += __popc(all);
+    if (all != 0xffffffffu) break;
+  }
+  if (before == 0) return false;
+  t->b = before - 1;
+  int last;
+  seq_rows(a, t->b, t->first, last);
+  t->n = last - t->first;
+  t->first_row = (id - (int)((int64_t)t->first * group / T + t->b)) * T;
+  t->rows = min(T, t->n * group - t->first_row);
+  if (t->rows <= 0 || t->first_row < 0) return false;   // (below zero only where row_start decreases)
+  const int64_t most = (int64_t)a.max_pages * a.page_size;
+  t->len = (int)max((int64_t)0, min((int64_t)table_at(a.kv_len, t->b), most));
+  return true;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_fast(float x) {   // 2 ulp; 0 for -inf
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t half2_bits(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Bytes `sel` of w (each xored with 0x80 beforehand: v + 128) as two fp16 numbers: 0x6400 is 1024 with a
+// last place of 1, so 1024 + 128 + v is exact and so is its difference from 1152.
+__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t w, uint32_t sel) {
+  const uint32_t t = __byte_perm(w, 0x64646464u, sel);
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&t), __floats2half2_rn(1152.0f, 1152.0f));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // 2^e, e in -126..127
+
 cudaError_t launch_kv_io(const KvArgs& a, void* k, void* v, int dtype, int64_t ld, bool append, cudaStream_t s);
 cudaError_t launch_kv_attention(const KvArgs& a, const AttendArgs& t, int dtype, cudaStream_t s);
+// the many-row kernel on tcgen05: kv_attention_tcgen05.cu
+cudaError_t launch_kv_attend_many(const KvArgs& a, const AttendArgs& t, int dtype, cudaStream_t s);
+int kv_attend_many_setup(std::string* why);
 
 }  // namespace sdq

@@ -314,6 +314,7 @@ int sdq_init(int device) {
   int rc = qgemm_tc_setup(&why);
   if (rc == SDQ_OK) rc = fgemm_setup(&why);
   if (rc == SDQ_OK) rc = sdpa_setup(&why);
+  if (rc == SDQ_OK) rc = kv_attend_many_setup(&why);
   if (rc != SDQ_OK) { cudaFree(c->status); delete c; return fail(rc, why); }
   g_ctx = c;
   return SDQ_OK;
@@ -946,12 +947,14 @@ int sdq_kv_attention(const sdq_kv_cache* cache, const sdq_kv_seqs* seqs, const v
     const int64_t width = (int64_t)heads * a.D;
     AttendArgs t;
     t.q = q_dev; t.out = out_dev; t.ldq = ldq ? ldq : width; t.ldo = ldo ? ldo : width;
+    t.status = nullptr;
     t.heads = heads; t.causal = (flags & SDQ_CAUSAL) ? 1 : 0; t.scale = scale;
     if (t.ldq < width || t.ldo < width) return invalid(kName, "a row stride is shorter than a row");
     if (!natural(q_dev, dtype) || !natural(out_dev, dtype)) return invalid(kName, "a pointer is not aligned to its element");
     DeviceGuard g;
     if (int rc = g.enter()) return rc;
     if (none) return SDQ_OK;
+    t.status = g_ctx->status;
     return launched(kName, launch_kv_attention(a, t, dtype, (cudaStream_t)stream), flags, stream);
   });
 }
