@@ -1,22 +1,31 @@
 // Attention of many new rows over the paged int8 cache, on tcgen05.
 //
 // One CTA per (128 rows, cache head); a row is a (token, query head) pair, so the heads that share a
-// cache head fill one tile together.  14 warps:
+// cache head fill one tile together.  20 warps, in warpgroups of their own register counts:
 //   warps 0..7   : softmax, one thread per row and half of a block's 128 keys (two threads share a row)
-//   warps 8..11  : converters: the cache's int8 pages -> fp16 operand tiles in shared memory
-//   warp 12      : MMA issuer of the scores, S = Q K^T, Q as A operand in tensor memory
-//   warp 13      : MMA issuer of O += P V, P in tensor memory (written in place over S)
-// Tensor memory (512 columns): Q hi 0..63, Q lo 64..127, O 128..255, S / P buffers 256..383, 384..511.
+//   warps 8..11  : converters of keys: the cache's int8 pages -> fp16 operand tiles in shared memory
+//   warps 12..15 : converters of values, transposed on the way
+//   warp 16      : MMA issuer of the scores, S = Q K^T
+//   warp 17      : MMA issuer of O += P V, P in tensor memory (written in place over S)
+// S is double-buffered in tensor memory, so the softmax of a block overlaps the products of its neighbours.
+//
+// bf16 and fp16 queries: the two halves of a block's keys are two independent attentions, each with running
+// offsets, sums and an O of its own (tensor memory: O 0..127 and 128..255, S / P 256..383 and 384..511; Q in
+// shared memory), which meet at the end; the two groups of softmax warps never wait for each other, and one's
+// exponentials run beside the other's maxima.  fp32 queries have two fp16 numbers per element of Q and of
+// the weights and need shared memory to add O up in (see below): Q lies in tensor memory (hi 0..63, lo
+// 64..127), there is one O (128..255), and the two threads of a row agree on every block's maximum.
 //
 // The cached integers are exact in fp16, so a product takes one MMA for each fp16 number that the other
 // factor is made of: one for bf16 and fp16 queries, two (hi + lo, 22 bits) for fp32 ones.  The keys' scales
 // enter with the scores and the values' with the weights, w = p * v_scale / 2^ev, where 2^ev bounds the
 // sequence's v scales (found in a pass over them: 4 of the 2 (D + 4) bytes of a key).
 //
-// Softmax in one sweep with a running offset m of each row: p = 2^10 2^(s - m); the offset moves, and O and
-// the row's sum are scaled down, only when a block's maximum exceeds it by more than 4 log2 units, so a
-// weight stays below 2^14 and inside fp16.  The two threads of a row agree on a block's maximum through
-// shared memory.  With fp32 queries O is taken out of tensor memory every kDrain blocks and added up in
+// Softmax in one sweep with a running offset m of each row: p = 2^6 2^(s - m); the offset moves, and O and
+// the row's sum are scaled down, only when a block's maximum exceeds it by more than 9 log2 units, so a
+// weight stays below 2^15 and inside fp16, whose grid ends at 2^-31 of the weight at the offset.  (With 4
+// units a fifth of the blocks had some row of a warp that moved, and scaling O costs as much as a block's
+// exponentials.)  With fp32 queries O is taken out of tensor memory every kDrain blocks and added up in
 // shared memory in fp32: the tensor core's accumulator truncates, and over thousands of keys that would be
 // the largest error there is (1e-5 of the result at 4k keys).
 //
@@ -34,27 +43,30 @@ using namespace tc;
 constexpr int kRowsT = 128;        // rows of a tile
 constexpr int kKeys = 128;         // keys of a block
 constexpr int kPlane = kKeys * 128 * 2;        // 32 KiB: a block's keys or values in fp16
-constexpr int kThreadsT = 448;
+constexpr int kThreadsT = 640;
+// registers of a thread: 640 threads are launched with 96 each; 256 * 144 + 256 * 72 + 128 * 40 = 60416 of 61440
+constexpr int kRegsSoftmax = 144, kRegsConvert = 72, kRegsIssue = 40;
 constexpr int kDrain = 4;          // blocks between two drains of O (fp32 queries)
-constexpr uint32_t kColQhi = 0, kColQlo = 64, kColO = 128, kColS = 256;
-constexpr float kShift = 10.0f;    // weights are 2^10 times p
-constexpr float kStepUp = 4.0f;    // log2 units by which a block's maximum may exceed the running offset
+constexpr uint32_t kColQhi = 0, kColQlo = 64, kColS = 256;
+__host__ __device__ constexpr uint32_t kColO(int planes, int grp) { return planes == 2 ? 128u : 128u * grp; }
+constexpr float kShift = 6.0f;     // weights are 2^6 times p
+constexpr float kStepUp = 9.0f;    // log2 units by which a block's maximum may exceed the running offset
 
 // Shared memory behind the operand tiles.
 struct Book {
   float ks[4][kKeys], vs[4][kKeys];   // scales of the blocks under way
   uint32_t there[4][4];               // which of their keys exist
-  int rows[4][kKeys];                 // pool rows
+  int rows[2][4][kKeys];              // pool rows, as the converters of keys and of values looked them up
   float meet[2][2][kRowsT];           // what the two threads of a row tell each other
-  float sum[2][kRowsT];
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pready[2], pvdone[2], scales[4], qready, lready, ofull, pair[4];
+  float sum[2][kRowsT], off[2][kRowsT];   // sums and offsets of the two halves
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pready[2][2], pvdone[2][2], scales[4], qready, lready, ofull, pair[4];
   uint32_t v_top;
   uint32_t tmem;
   int abort;
 };
 constexpr int kSlack = 1024;       // to bring the dynamic base to a 1024-byte boundary
 template <int P>
-constexpr int kSmemMany = 4 * kPlane + (P == 2 ? 128 * kRowsT * 4 : 0) + (int)sizeof(Book) + kSlack;
+constexpr int kSmemMany = 4 * kPlane + (P == 2 ? 128 * kRowsT * 4 : kPlane) + (int)sizeof(Book) + kSlack;
 
 __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -62,6 +74,14 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
       "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -97,8 +117,9 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw);
   const uint32_t smem_v = base + 2 * kPlane;
-  float* drained = reinterpret_cast<float*>(smem + 4 * kPlane);   // [d][row], fp32 queries
-  Book& bk = *reinterpret_cast<Book*>(smem + 4 * kPlane + (P == 2 ? 128 * kRowsT * 4 : 0));
+  const uint32_t smem_q = base + 4 * kPlane;                      // 16-bit queries: q as operand tile
+  float* drained = reinterpret_cast<float*>(smem + 4 * kPlane);   // fp32 queries: [d][row], O so far
+  Book& bk = *reinterpret_cast<Book*>(smem + 4 * kPlane + (P == 2 ? 128 * kRowsT * 4 : kPlane));
   volatile int* abort_flag = &bk.abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kh = blockIdx.y, group = t.heads / a.heads;
@@ -124,8 +145,10 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
       mbar_init(bar(bk.vfull[i]), 4);
       mbar_init(bar(bk.vempty[i]), 1);
       mbar_init(bar(bk.sfull[i]), 1);
-      mbar_init(bar(bk.pready[i]), 8);
-      mbar_init(bar(bk.pvdone[i]), 1);
+      for (int h = 0; h < 2; h++) {
+        mbar_init(bar(bk.pready[i][h]), P == 2 ? 8 : 4);
+        mbar_init(bar(bk.pvdone[i][h]), 1);
+      }
     }
     for (int i = 0; i < 4; i++) {
       mbar_init(bar(bk.scales[i]), 4);
@@ -139,7 +162,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 12) {
+  if (warp == 16) {
     tmem_alloc(smem_u32(&bk.tmem), 512);
     tmem_relinquish();
   }
@@ -166,46 +189,29 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
   const uint32_t tmem_base = bk.tmem;
   const int ev = min(max((int)(bk.v_top >> 23) - 126, -126), 126);   // v_scale < 2^ev (where it is finite)
 
+  auto key_of = [&](int j) { return j < nblk ? place(j * kKeys + (int)(threadIdx.x & 127)) : -1; };
   if (warp >= 8 && warp < 12) {
-    // ---------------------------------------------------------------- converters
-    const int w = warp - 8, tt = threadIdx.x - 256;       // 0..127
-    const int piece = tt & 7, krow = tt >> 3;             // keys: 16 bytes of d, key krow + 16 i
-    const int dw = lane & 7, kg = lane >> 3;              // values: 4 of this warp's 32 values of d, 8 of 32 keys
-    const bool has_k = piece * 16 < a.D, has_v = 32 * w + 4 * dw < a.D;
+    // ---------------------------------------------------------------- converters of keys
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
+    const int tt = threadIdx.x & 127;
+    const int piece = tt & 7, krow = tt >> 3;             // 16 bytes of d, key krow + 16 i
+    const bool has_k = piece * 16 < a.D;
     const float unit = pow2f(-ev);
-    auto key_of = [&](int j) { return j < nblk ? place(j * kKeys + tt) : -1; };
     uint4 kr[8];
-    uint32_t vr[4][8];
     auto load_k = [&](int j) {
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        const int row = bk.rows[j & 3][krow + 16 * i];
+        const int row = bk.rows[0][j & 3][krow + 16 * i];
         kr[i] = make_uint4(0, 0, 0, 0);
         if (row >= 0 && has_k) kr[i] = __ldg(reinterpret_cast<const uint4*>(a.k + (int64_t)row * a.D + piece * 16));
       }
     };
-    auto load_v = [&](int j) {
-#pragma unroll
-      for (int it = 0; it < 4; it++) {
-        const int4* rp = reinterpret_cast<const int4*>(&bk.rows[j & 3][it * 32 + kg * 8]);
-        const int4 r0 = rp[0], r1 = rp[1];
-        const int rows[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          vr[it][e] = 0;
-          if (rows[e] >= 0 && has_v) vr[it][e] = __ldg(reinterpret_cast<const uint32_t*>(a.v + (int64_t)rows[e] * a.D + 32 * w + 4 * dw));
-        }
-      }
-    };
     int row_now = key_of(0), row_next = key_of(1);
-    bk.rows[0][tt] = row_now;
-    bk.rows[1][tt] = row_next;
+    bk.rows[0][0][tt] = row_now;
+    bk.rows[0][1][tt] = row_next;
     float ks = row_now >= 0 ? __ldg(a.k_scale + row_now) : 0.0f, vs = row_now >= 0 ? __ldg(a.v_scale + row_now) : 0.0f;
     asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (nblk > 0) {
-      load_k(0);
-      load_v(0);
-    }
+    if (nblk > 0) load_k(0);
     bool ok = true;   // after a wait that gave up the loop only keeps the warps' meetings
     for (int j = 0; j < nblk; j++) {
       const int row_2 = key_of(j + 2);
@@ -236,35 +242,69 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
         bk.ks[j & 3][tt] = ks;
         bk.vs[j & 3][tt] = vs * unit;
         const uint32_t there = __ballot_sync(0xffffffffu, row_now >= 0);
-        if (lane == 0) bk.there[j & 3][w] = there;
+        if (lane == 0) bk.there[j & 3][warp - 8] = there;
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(bar(bk.kfull[slot]));
           mbar_arrive(bar(bk.scales[j & 3]));
         }
-        if (j + 1 < nblk) load_k(j + 1);
+        if (j + 1 < nblk) load_k(j + 1);   // behind the fence, which would wait for it
       }
+      row_now = row_next;
+      row_next = row_2;
+      bk.rows[0][(j + 2) & 3][tt] = row_2;
+      ks = row_now >= 0 ? __ldg(a.k_scale + row_now) : 0.0f;
+      vs = row_now >= 0 ? __ldg(a.v_scale + row_now) : 0.0f;
+      asm volatile("bar.sync 1, 128;" ::: "memory");   // the next rows are there
+    }
+  } else if (warp >= 12 && warp < 16) {
+    // ---------------------------------------------------------------- converters of values
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
+    const int w = warp - 12, tt = threadIdx.x & 127;
+    const int piece = lane & 7, kg = lane >> 3;           // 16 values of d of 8 of this warp's 32 keys
+    const bool has_v = piece * 16 < a.D;
+    uint4 vr[8];
+    auto load_v = [&](int j) {
+      const int4* rp = reinterpret_cast<const int4*>(&bk.rows[1][j & 3][w * 32 + kg * 8]);
+      const int4 r0 = rp[0], r1 = rp[1];
+      const int rows[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        vr[e] = make_uint4(0, 0, 0, 0);
+        if (rows[e] >= 0 && has_v) vr[e] = __ldg(reinterpret_cast<const uint4*>(a.v + (int64_t)rows[e] * a.D + piece * 16));
+      }
+    };
+    bk.rows[1][0][tt] = key_of(0);
+    bk.rows[1][1][tt] = key_of(1);
+    asm volatile("bar.sync 2, 128;" ::: "memory");
+    if (nblk > 0) load_v(0);
+    bool ok = true;
+    for (int j = 0; j < nblk; j++) {
+      const int row_2 = key_of(j + 2);
+      const uint32_t slot = j & 1, ph = (j >> 1) & 1;
       ok = ok && mbar_wait_warp(bar(bk.vempty[slot]), ph ^ 1u, abort_flag, t.status, 0xc00 | 2);
       if (ok) {
-        if (32 * w < a.D) {
+        if (has_v) {
+          const uint32_t st = smem_v + slot * kPlane + (w >> 1) * 16384;
+          const int chunk = (w & 1) * 4 + kg;
 #pragma unroll
-          for (int it = 0; it < 4; it++) {
+          for (int q = 0; q < 4; q++) {
             uint32_t h[4][4];   // [value of d][pair of keys]
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
-              const uint32_t x = __byte_perm(vr[it][e], vr[it][e + 1], 0x5140) ^ 0x80808080u;
-              const uint32_t y = __byte_perm(vr[it][e], vr[it][e + 1], 0x7362) ^ 0x80808080u;
+              const uint32_t u = q == 0 ? vr[e].x : q == 1 ? vr[e].y : q == 2 ? vr[e].z : vr[e].w;
+              const uint32_t v = q == 0 ? vr[e + 1].x : q == 1 ? vr[e + 1].y : q == 2 ? vr[e + 1].z : vr[e + 1].w;
+              const uint32_t x = __byte_perm(u, v, 0x5140) ^ 0x80808080u, y = __byte_perm(u, v, 0x7362) ^ 0x80808080u;
               h[0][e / 2] = bytes_to_half2(x, 0x4140);
               h[1][e / 2] = bytes_to_half2(x, 0x4342);
               h[2][e / 2] = bytes_to_half2(y, 0x4140);
               h[3][e / 2] = bytes_to_half2(y, 0x4342);
             }
-            const int chunk = (it & 1) * 4 + kg;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-              const int d = 32 * w + 4 * dw + i;
-              st_shared_v4_b32(smem_v + slot * kPlane + (it >> 1) * 16384 + d * 128 + ((chunk ^ (d & 7)) << 4), h[i][0], h[i][1], h[i][2], h[i][3]);
+              const int d = 16 * piece + 4 * q + i;
+              st_shared_v4_b32(st + d * 128 + ((chunk ^ (d & 7)) << 4), h[i][0], h[i][1], h[i][2], h[i][3]);
             }
           }
         }
@@ -273,61 +313,69 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
         if (lane == 0) mbar_arrive(bar(bk.vfull[slot]));
         if (j + 1 < nblk) load_v(j + 1);
       }
-      row_now = row_next;
-      row_next = row_2;
-      bk.rows[(j + 2) & 3][tt] = row_2;
-      ks = row_now >= 0 ? __ldg(a.k_scale + row_now) : 0.0f;
-      vs = row_now >= 0 ? __ldg(a.v_scale + row_now) : 0.0f;
-      asm volatile("bar.sync 1, 128;" ::: "memory");   // the next rows are there
+      bk.rows[1][(j + 2) & 3][tt] = row_2;
+      asm volatile("bar.sync 2, 128;" ::: "memory");
     }
-  } else if (warp == 12) {
-    if (lane == 0 && nblk > 0) {
+  } else if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+    if (warp == 16 && lane == 0 && nblk > 0) {
       // -------------------------------------------------------------- scores
       constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kRowsT >> 4) << 24);
       bool ok = mbar_wait_spin(bar(bk.qready), 0, abort_flag, t.status, 0xc00 | 3);
       for (int j = 0; ok && j < nblk; j++) {
         const uint32_t slot = j & 1, ph = (j >> 1) & 1;
         ok = mbar_wait_spin(bar(bk.kfull[slot]), ph, abort_flag, t.status, 0xc00 | 4);
-        if (ok && j >= 2) ok = mbar_wait_spin(bar(bk.pvdone[slot]), ph ^ 1u, abort_flag, t.status, 0xc00 | 5);
+        if (ok && j >= 2) ok = mbar_wait_spin(bar(bk.pvdone[slot][0]), ph ^ 1u, abort_flag, t.status, 0xc00 | 5);
+        if (P == 1 && ok && j >= 2) ok = mbar_wait_spin(bar(bk.pvdone[slot][1]), ph ^ 1u, abort_flag, t.status, 0xc00 | 5);
         if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem_base + kColS + slot * kKeys, st = base + slot * kPlane;
         for (int ks = 0; ks < a.D / 16; ks++) {
           const uint64_t k = make_smem_desc(st + (ks >> 2) * 16384) + (uint64_t)((ks & 3) * 2);
-          if constexpr (P == 2) umma_f16_ts(d, tmem_base + kColQlo + ks * 8, k, kIdesc, ks != 0);
-          umma_f16_ts(d, tmem_base + kColQhi + ks * 8, k, kIdesc, P == 2 || ks != 0);
+          if constexpr (P == 2) {
+            umma_f16_ts(d, tmem_base + kColQlo + ks * 8, k, kIdesc, ks != 0);
+            umma_f16_ts(d, tmem_base + kColQhi + ks * 8, k, kIdesc, 1u);
+          } else {
+            umma_f16_ss(d, make_smem_desc(smem_q + (ks >> 2) * 16384) + (uint64_t)((ks & 3) * 2), k, kIdesc, ks != 0);
+          }
         }
         umma_commit(bar(bk.kempty[slot]));
         umma_commit(bar(bk.sfull[slot]));
       }
     }
-  } else if (warp == 13) {
-    if (lane == 0 && nblk > 0) {
+    if (warp == 17 && lane == 0 && nblk > 0) {
       // -------------------------------------------------------------- P V
       const uint32_t idesc = (1u << 4) | ((uint32_t)(a.D >> 3) << 17) | ((uint32_t)(kRowsT >> 4) << 24);
       bool ok = true;
       for (int j = 0; ok && j < nblk; j++) {
         const uint32_t slot = j & 1, ph = (j >> 1) & 1;
-        ok = mbar_wait_spin(bar(bk.pready[slot]), ph, abort_flag, t.status, 0xc00 | 6);
-        if (ok) ok = mbar_wait_spin(bar(bk.vfull[slot]), ph, abort_flag, t.status, 0xc00 | 7);
-        if (!ok) break;
-        tc_fence_after();
+        ok = mbar_wait_spin(bar(bk.vfull[slot]), ph, abort_flag, t.status, 0xc00 | 7);
         const bool fresh = P == 2 ? j % kDrain == 0 : j == 0;   // O was taken out (or is new)
         const uint32_t p0 = tmem_base + kColS + slot * kKeys;
+        for (int h = 0; ok && h < (P == 2 ? 1 : 2); h++) {
+          ok = mbar_wait_spin(bar(bk.pready[slot][h]), ph, abort_flag, t.status, 0xc00 | 6);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t o = tmem_base + kColO(P, h);
+          constexpr int kSteps = P == 2 ? kKeys / 16 : kKeys / 32;
 #pragma unroll
-        for (int ks = 0; ks < kKeys / 16; ks++) {
-          const uint64_t v = make_smem_desc(smem_v + slot * kPlane + (ks >> 2) * 16384) + (uint64_t)((ks & 3) * 2);
-          // the weights of keys 32 c + 16 i .. lie in 8 columns: hi at 32 c + 8 i, lo 16 further
-          const uint32_t p = p0 + (ks >> 1) * 32 + (ks & 1) * 8;
-          if constexpr (P == 2) umma_f16_ts(tmem_base + kColO, p + 16, v, idesc, !(fresh && ks == 0));
-          umma_f16_ts(tmem_base + kColO, p, v, idesc, P == 2 || !(fresh && ks == 0));
+          for (int i = 0; i < kSteps; i++) {
+            const int ks = h * kSteps + i;
+            const uint64_t v = make_smem_desc(smem_v + slot * kPlane + (ks >> 2) * 16384) + (uint64_t)((ks & 3) * 2);
+            // the weights of keys 32 c + 16 i .. lie in 8 columns: hi at 32 c + 8 i, lo 16 further
+            const uint32_t p = p0 + (ks >> 1) * 32 + (ks & 1) * 8;
+            if constexpr (P == 2) umma_f16_ts(o, p + 16, v, idesc, !(fresh && i == 0));
+            umma_f16_ts(o, p, v, idesc, P == 2 || !(fresh && i == 0));
+          }
+          umma_commit(bar(bk.pvdone[slot][h]));
         }
+        if (!ok) break;
         umma_commit(bar(bk.vempty[slot]));
-        umma_commit(bar(bk.pvdone[slot]));
       }
       if (ok) umma_commit(bar(bk.ofull));
     }
-  } else if (warp < 8) {
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     // ---------------------------------------------------------------- softmax
     const int quarter = warp & 3, grp = warp >> 2, r = quarter * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
@@ -381,15 +429,20 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
       uint32_t hi[32];
 #pragma unroll
       for (int i = 0; i < 32; i++) hi[i] = half2_bits(q[2 * i] * inv, q[2 * i + 1] * inv);
-      tmem_st_32x32(tmem_base + kColQhi + grp * 32 + lane_base, hi);
       if constexpr (P == 2) {
+        tmem_st_32x32(tmem_base + kColQhi + grp * 32 + lane_base, hi);
         uint32_t lo[32];
 #pragma unroll
         for (int i = 0; i < 32; i++) lo[i] = rest_bits(hi[i], q[2 * i] * inv, q[2 * i + 1] * inv);
         tmem_st_32x32(tmem_base + kColQlo + grp * 32 + lane_base, lo);
+        tmem_st_wait();
+        tc_fence_before();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          st_shared_v4_b32(smem_q + grp * 16384 + r * 128 + ((i ^ (r & 7)) << 4), hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+        fence_async_smem();
       }
-      tmem_st_wait();
-      tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(bk.qready));
     }
@@ -413,7 +466,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
       for (int h = 0; h < 2; h++)
         sees[h] = bk.there[j & 3][grp * 2 + h] & (left >= 32 * h + 32 ? 0xffffffffu : left <= 32 * h ? 0u : (1u << (left - 32 * h)) - 1);
       const bool all = __all_sync(0xffffffffu, (sees[0] & sees[1]) == 0xffffffffu);
-      float bm = -INFINITY;
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // independent chains
 #pragma unroll
       for (int h = 0; h < 2; h++) {
 #pragma unroll
@@ -429,12 +482,15 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
             if (!((sees[h] >> i) & 1)) s[h][i] = 0xff800000u;   // -inf
         }
 #pragma unroll
-        for (int i = 0; i < 32; i++) bm = fmaxf(bm, __uint_as_float(s[h][i]));
+        for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[h][i]));
       }
-      bk.meet[j & 1][grp][r] = bm;    // alternating, so that one meeting a block is enough
-      ok = pair_sync();
-      if (!ok) break;
-      bm = fmaxf(bm, bk.meet[j & 1][grp ^ 1][r]);
+      float bm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      if constexpr (P == 2) {
+        bk.meet[j & 1][grp][r] = bm;    // alternating, so that one meeting a block is enough
+        ok = pair_sync();
+        if (!ok) break;
+        bm = fmaxf(bm, bk.meet[j & 1][grp ^ 1][r]);
+      }
       const bool grow = (bm - m) * factor > kStepUp;   // true in the row's first block with a key
       const bool drain = P == 2 && j > 0 && j % kDrain == 0;
       const bool any = __any_sync(0xffffffffu, grow);
@@ -449,14 +505,14 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
         if (j > 0) {
           // O holds the blocks so far: the last P V must be done before O is scaled or taken out (the
           // next one waits for this block's weights)
-          ok = mbar_wait_warp(bar(bk.pvdone[(j - 1) & 1]), ((j - 1) >> 1) & 1, abort_flag, t.status, 0xc00 | 11);
+          ok = mbar_wait_warp(bar(bk.pvdone[(j - 1) & 1][P == 2 ? 0 : grp]), ((j - 1) >> 1) & 1, abort_flag, t.status, 0xc00 | 11);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 2 * grp; c < 2 * grp + 2; c++) {
+          for (int c = P == 2 ? 2 * grp : 0; c < (P == 2 ? 2 * grp + 2 : 4); c++) {
             if (c * 32 >= a.D) break;
             uint32_t o[32];
-            tmem_ld_32x32(tmem_base + kColO + c * 32 + lane_base, o);
+            tmem_ld_32x32(tmem_base + kColO(P, grp) + c * 32 + lane_base, o);
             tmem_ld_wait();
             if constexpr (P == 2) {
               float* d = drained + c * 32 * kRowsT + r;
@@ -472,31 +528,32 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
             }
 #pragma unroll
             for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st_32x32(tmem_base + kColO + c * 32 + lane_base, o);
+            tmem_st_32x32(tmem_base + kColO(P, grp) + c * 32 + lane_base, o);
           }
         }
       }
-      float lb[2] = {};   // the block's sum by itself: fewer roundings than one long chain
+      float lb[4] = {};   // the block's sum by itself: fewer roundings than one long chain
       // each 32 columns of scores become 16 of fp16 pairs of weights (hi), then 16 of what is left (lo)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         uint32_t hi[32];
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const float4 v4 = vs[h * 8 + i / 4];
-          const float vv[4] = {v4.x, v4.y, v4.z, v4.w};
-          float wt[4];
+        for (int i = 0; i < 32; i += 8) {
+          const float4 va = vs[h * 8 + i / 4], vb = vs[h * 8 + i / 4 + 1];
+          const float vv[8] = {va.x, va.y, va.z, va.w, vb.x, vb.y, vb.z, vb.w};
+          float p[8];
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float p = exp2_fast(fmaf(__uint_as_float(s[h][i + e]), factor, e_off));
-            lb[e & 1] += p;
-            wt[e] = p * vv[e];
+          for (int e = 0; e < 8; e++) p[e] = exp2_fast(fmaf(__uint_as_float(s[h][i + e]), factor, e_off));
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            lb[e & 3] += p[e];
+            p[e] *= vv[e];
           }
 #pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            const uint32_t x = half2_bits(wt[e], wt[e + 1]);
+          for (int e = 0; e < 8; e += 2) {
+            const uint32_t x = half2_bits(p[e], p[e + 1]);
             hi[(i + e) / 2] = x;
-            if constexpr (P == 2) hi[16 + (i + e) / 2] = rest_bits(x, wt[e], wt[e + 1]);
+            if constexpr (P == 2) hi[16 + (i + e) / 2] = rest_bits(x, p[e], p[e + 1]);
           }
         }
         if constexpr (P == 2) {
@@ -508,15 +565,16 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
           tmem_st_32x16(s_col + 32 * h, h16);
         }
       }
-      l += lb[0] + lb[1];
+      l += (lb[0] + lb[1]) + (lb[2] + lb[3]);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(bk.pready[slot]));
+      if (lane == 0) mbar_arrive(bar(bk.pready[slot][P == 2 ? 0 : grp]));
     }
     // ---- both halves' sums, then O / l ----
     if (ok) {
       bk.sum[grp][r] = l;
+      bk.off[grp][r] = m;
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(bk.lready));
       ok = mbar_wait_warp(bar(bk.lready), 0, abort_flag, t.status, 0xc00 | 12);
@@ -524,7 +582,14 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
     if (ok && nblk > 0) ok = mbar_wait_warp(bar(bk.ofull), 0, abort_flag, t.status, 0xc00 | 13);
     if (ok) {
       tc_fence_after();
-      l = bk.sum[0][r] + bk.sum[1][r];
+      float f[2] = {1.0f, 1.0f};   // brings the halves to one offset
+      if constexpr (P == 1) {
+        const float top = fmaxf(bk.off[0][r], bk.off[1][r]);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          if (top != -INFINITY) f[h] = exp2_fast((bk.off[h][r] - top) * factor);
+      }
+      l = bk.sum[0][r] * f[0] + bk.sum[1][r] * f[1];
       const float inv = l != 0.0f ? (1.0f / l) * pow2f(ev) : 0.0f;   // a row that sees no key is zero
       const int64_t at = (int64_t)(tile.first + token) * t.ldo + (int64_t)head * a.D;
 #pragma unroll 1
@@ -533,11 +598,18 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
         float o[32];
         if (nblk > 0) {
           uint32_t x[32];
-          tmem_ld_32x32(tmem_base + kColO + c * 32 + lane_base, x);
+          tmem_ld_32x32(tmem_base + kColO(P, 0) + c * 32 + lane_base, x);
           tmem_ld_wait();
 #pragma unroll
+          for (int i = 0; i < 32; i++) o[i] = __uint_as_float(x[i]) * f[0];
+          if constexpr (P == 1) {
+            tmem_ld_32x32(tmem_base + kColO(P, 1) + c * 32 + lane_base, x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] += __uint_as_float(x[i]) * f[1];
+          }
+#pragma unroll
           for (int i = 0; i < 32; i++) {
-            o[i] = __uint_as_float(x[i]);
             if constexpr (P == 2) {
               if (nblk > kDrain) o[i] += drained[(c * 32 + i) * kRowsT + r];
             }
@@ -575,7 +647,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
     for (int i = 0; i < 1000; i++) __nanosleep(1000);   // let MMAs in flight end (~1 ms)
     __syncthreads();
   }
-  if (warp == 12) {
+  if (warp == 16) {
     __syncwarp();
     tmem_dealloc(tmem_base, 512);
   }
