@@ -11,14 +11,33 @@ namespace sdq {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kMaxTokens = 64;  // tokens of a block: as many as give each lane group a row
+constexpr int kMaxTokens = 64;
+// Rows of D values that a group of lanes has under way, and how many times it goes round.  Appending and
+// reading fp32 are carried by the number of warps; reading into 16 bits, a third of the bytes to write, by
+// loads under way.  8001 rows of 24 x 64 fp32: append 27.5 us with one, 30.5 with four; read 28.3 and 35.9.
+// 100003 rows of 8 x 128 bf16: read 139 us with one, 117 with four (208 with a block for each token).
+template <int DT, bool APPEND>
+constexpr int kAtOnce = APPEND || DT == SDQ_F32 ? 1 : 4;
+template <int DT, bool APPEND>
+constexpr int kRounds = kAtOnce<DT, APPEND> == 1 ? 4 : 2;
 
 struct IoArgs {
   void* k;       // [rows, heads, D], `ld` elements from row to row
   void* v;
   int64_t ld;
+  PageDiv per_token;   // 2 * heads rows of D values make a token
   int tokens;    // of one block
   int vec;       // the dense rows are 16-byte aligned
+};
+// The i-th row of D values of a block: its token, whether it is of v, and its head.
+struct Item {
+  int token, is_v, head;
+  __device__ __forceinline__ Item(const KvArgs& a, const IoArgs& io, int i) {
+    token = (int)io.per_token.page((uint32_t)i);
+    const int rest = i - token * 2 * a.heads;
+    is_v = rest >= a.heads;
+    head = rest - (is_v ? a.heads : 0);
+  }
 };
 
 template <int DT>
@@ -69,38 +88,52 @@ __device__ __forceinline__ void find_slots(const KvArgs& a, const IoArgs& io, in
 template <int DT, int LPR>
 __global__ void __launch_bounds__(kBlock) kv_append_kernel(const KvArgs a, const IoArgs io) {
   __shared__ int slot[kMaxTokens];
+  constexpr int kGroups = kBlock / LPR, U = kAtOnce<DT, true>;
   allow_dependent_launch();
   wait_prior_grids();
   find_slots(a, io, slot);
   const int part = threadIdx.x % LPR;
   const bool mine = part * 8 < a.D;
   const int items = io.tokens * 2 * a.heads;
-  for (int i0 = 0; i0 < items; i0 += kBlock / LPR) {   // whole warps go round together
-    const int i = i0 + threadIdx.x / LPR;
-    const int token = i / (2 * a.heads), rest = i - token * 2 * a.heads;
-    const int is_v = rest >= a.heads, head = rest - is_v * a.heads;
-    const int s = i < items ? slot[token] : -1;
-    float x[8] = {};
-    if (s >= 0 && mine) {
-      const int64_t row = (int64_t)blockIdx.x * io.tokens + token;
-      load8<DT>(is_v ? io.v : io.k, row * io.ld + head * a.D + part * 8, io.vec, x);
+  for (int i0 = threadIdx.x / LPR; i0 - (int)(threadIdx.x / LPR) < items; i0 += kGroups * U) {   // whole warps go round together
+    float x[U][8];
+    int64_t at[U];
+    bool is_v[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = i0 + u * kGroups;
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[u][e] = 0.0f;
+      at[u] = -1;
+      if (i < items) {
+        const Item it(a, io, i);
+        const int s = slot[it.token];
+        if (s >= 0) {
+          at[u] = (int64_t)s + (int64_t)it.head * a.page_size;
+          is_v[u] = it.is_v;
+          const int64_t row = (int64_t)blockIdx.x * io.tokens + it.token;
+          if (mine) load8<DT>(it.is_v ? io.v : io.k, row * io.ld + it.head * a.D + part * 8, io.vec, x[u]);
+        }
+      }
     }
-    float mx = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; e++) mx = fold_abs(mx, x[e]);
+    for (int u = 0; u < U; u++) {
+      float mx = 0.0f;
 #pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float sc = int8_row_scale(mx);
-    const float inv = __fdiv_rn(1.0f, sc);
-    if (s >= 0) {
-      const int64_t at = (int64_t)s + (int64_t)head * a.page_size;
-      if (part == 0) (is_v ? a.v_scale : a.k_scale)[at] = sc;
-      if (mine) {
-        int q[8];
+      for (int e = 0; e < 8; e++) mx = fold_abs(mx, x[u][e]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) q[e] = act_round(__fmul_rn(x[e], inv));
-        *reinterpret_cast<uint2*>((is_v ? a.v : a.k) + at * a.D + part * 8) =
-            make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+      for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float sc = int8_row_scale(mx);
+      const float inv = __fdiv_rn(1.0f, sc);
+      if (at[u] >= 0) {
+        if (part == 0) (is_v[u] ? a.v_scale : a.k_scale)[at[u]] = sc;
+        if (mine) {
+          int q[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) q[e] = act_round(__fmul_rn(x[u][e], inv));
+          *reinterpret_cast<uint2*>((is_v[u] ? a.v : a.k) + at[u] * a.D + part * 8) =
+              make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+        }
       }
     }
   }
@@ -111,6 +144,7 @@ __global__ void __launch_bounds__(kBlock) kv_append_kernel(const KvArgs a, const
 template <int DT, int LPR>
 __global__ void __launch_bounds__(kBlock) kv_read_kernel(const KvArgs a, const IoArgs io) {
   __shared__ int slot[kMaxTokens];
+  constexpr int kGroups = kBlock / LPR, U = kAtOnce<DT, false>;
   allow_dependent_launch();
   wait_prior_grids();
   find_slots(a, io, slot);
@@ -118,30 +152,48 @@ __global__ void __launch_bounds__(kBlock) kv_read_kernel(const KvArgs a, const I
   if (part * 8 >= a.D) return;
   const int first = __ldg(a.row_start), last = __ldg(a.row_start + a.batch);
   const int items = io.tokens * 2 * a.heads;
-  for (int i = threadIdx.x / LPR; i < items; i += kBlock / LPR) {
-    const int token = i / (2 * a.heads), rest = i - token * 2 * a.heads;
-    const int is_v = rest >= a.heads, head = rest - is_v * a.heads;
-    const int64_t row = (int64_t)blockIdx.x * io.tokens + token;
-    if (row >= a.rows || row < first || row >= last) continue;
-    const int s = slot[token];
-    float x[8] = {};
-    if (s >= 0) {
-      const int64_t at = (int64_t)s + (int64_t)head * a.page_size;
-      const float sc = __ldg((is_v ? a.v_scale : a.k_scale) + at);
-      const uint2 w = __ldg(reinterpret_cast<const uint2*>((is_v ? a.v : a.k) + at * a.D + part * 8));
+  for (int i0 = threadIdx.x / LPR; i0 < items; i0 += kGroups * U) {
+    uint2 w[U];
+    float sc[U];
 #pragma unroll
-      for (int e = 0; e < 8; e++)
-        x[e] = __fmul_rn((float)(int8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3))), sc);
+    for (int u = 0; u < U; u++) {
+      const int i = i0 + u * kGroups;
+      w[u] = make_uint2(0, 0);
+      sc[u] = 0.0f;
+      if (i < items) {
+        const Item it(a, io, i);
+        const int s = slot[it.token];
+        if (s >= 0) {
+          const int64_t at = (int64_t)s + (int64_t)it.head * a.page_size;
+          sc[u] = __ldg((it.is_v ? a.v_scale : a.k_scale) + at);
+          w[u] = __ldcs(reinterpret_cast<const uint2*>((it.is_v ? a.v : a.k) + at * a.D + part * 8));
+        }
+      }
     }
-    store8<DT>(is_v ? io.v : io.k, row * io.ld + head * a.D + part * 8, io.vec, x);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = i0 + u * kGroups;
+      if (i >= items) break;
+      const Item it(a, io, i);
+      const int64_t row = (int64_t)blockIdx.x * io.tokens + it.token;
+      if (row >= a.rows || row < first || row >= last) continue;
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = __fmul_rn((float)(int8_t)((e < 4 ? w[u].x : w[u].y) >> (8 * (e & 3))), sc[u]);
+      store8<DT>(it.is_v ? io.v : io.k, row * io.ld + it.head * a.D + part * 8, io.vec, x);
+    }
   }
 }
 
 template <int DT, int LPR>
 cudaError_t launch_io(const KvArgs& a, IoArgs io, bool append, cudaStream_t s) {
-  const int lanes = 2 * a.heads * LPR;   // lane groups that one token fills
-  io.tokens = lanes >= kBlock ? 1 : kBlock / lanes;
+  // the rounds it takes, but no fewer than four blocks to an SM
+  const int rows = (append ? kRounds<DT, true> * kAtOnce<DT, true> : kRounds<DT, false> * kAtOnce<DT, false>) * (kBlock / LPR);
+  const int full = (rows + 2 * a.heads - 1) / (2 * a.heads);
+  const int spread = a.rows / (148 * 4);
+  io.tokens = full < spread ? full : spread;
   if (io.tokens > kMaxTokens) io.tokens = kMaxTokens;
+  if (io.tokens < 1) io.tokens = 1;
   const unsigned grid = (unsigned)(((int64_t)a.rows + io.tokens - 1) / io.tokens);
   return append ? launch_overlapped(kv_append_kernel<DT, LPR>, dim3(grid), dim3(kBlock), 0, s, a, io)
                 : launch_overlapped(kv_read_kernel<DT, LPR>, dim3(grid), dim3(kBlock), 0, s, a, io);
@@ -158,10 +210,9 @@ cudaError_t launch_typed(const KvArgs& a, const IoArgs& io, bool append, cudaStr
 }  // namespace
 
 cudaError_t launch_kv_io(const KvArgs& a, void* k, void* v, int dtype, int64_t ld, bool append, cudaStream_t s) {
-  IoArgs io;
-  io.k = k; io.v = v; io.ld = ld; io.tokens = 1;
   const int64_t per = dtype == SDQ_F32 ? 4 : 8;
-  io.vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0 && ld % per == 0;
+  const IoArgs io{k, v, ld, PageDiv(2u * (uint32_t)a.heads), 1,
+                  ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0 && ld % per == 0};
   count_launch();
   if (dtype == SDQ_F32) return launch_typed<SDQ_F32>(a, io, append, s);
   if (dtype == SDQ_BF16) return launch_typed<SDQ_BF16>(a, io, append, s);

@@ -477,6 +477,33 @@ __global__ void __launch_bounds__(kThreads) dequant_rows_kernel(const int8_t* __
     w[i] = __fmul_rn((float)q[i], scale[i / last]);
 }
 
+// The same for rows of a multiple of 4 elements and aligned pointers: 4 elements to a lane, 4 such pieces
+// under way.  27280 x 4096: 228 -> 96 us, of 86 at the measured copy rate.
+__global__ void __launch_bounds__(kThreads) dequant_rows_vec(const int8_t* __restrict__ q,
+                                                             const float* __restrict__ scale,
+                                                             uint32_t pieces, uint32_t per_row,
+                                                             float* __restrict__ w) {
+  allow_dependent_launch();
+  wait_prior_grids();
+  const uint32_t first = blockIdx.x * (4 * kThreads) + threadIdx.x;   // below 2^32: pieces <= 2^31
+  uint32_t x[4];
+  float sc[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t at = first + i * kThreads;
+    x[i] = at < pieces ? __ldcs(reinterpret_cast<const uint32_t*>(q) + at) : 0u;
+    sc[i] = at < pieces ? __ldg(scale + at / per_row) : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t at = first + i * kThreads;
+    if (at < pieces)
+      __stcs(reinterpret_cast<float4*>(w) + at,
+             make_float4(__fmul_rn((float)(int8_t)x[i], sc[i]), __fmul_rn((float)(int8_t)(x[i] >> 8), sc[i]),
+                         __fmul_rn((float)(int8_t)(x[i] >> 16), sc[i]), __fmul_rn((float)(int8_t)(x[i] >> 24), sc[i])));
+  }
+}
+
 template <int DT, int MODE>
 cudaError_t launch_quant_t(const void* src, int64_t rows, int64_t last, int8_t* q, float* scale,
                            int sm_count, cudaStream_t s) {
@@ -592,6 +619,13 @@ cudaError_t launch_dequant_rows(const int8_t* q, const float* scale, int64_t row
                                 float* w, int sm_count, cudaStream_t s) {
   const int64_t numel = rows * last;
   if (numel <= 0) return cudaSuccess;
+  if (last % 4 == 0 && numel / 4 <= (int64_t(1) << 31) && (reinterpret_cast<uintptr_t>(q) & 3) == 0 &&
+      (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
+    const uint32_t pieces = (uint32_t)(numel / 4);
+    count_launch();
+    return launch_overlapped(dequant_rows_vec, dim3((pieces + 4 * kThreads - 1) / (4 * kThreads)), dim3(kThreads), 0, s,
+                             q, scale, pieces, (uint32_t)(last / 4), w);
+  }
   int64_t blocks = (numel + kThreads - 1) / kThreads;
   if (blocks > (int64_t)sm_count * 16) blocks = (int64_t)sm_count * 16;
   count_launch();
