@@ -109,6 +109,32 @@ __device__ __forceinline__ uint32_t rest_bits(uint32_t hi, float x, float y) {  
   return half2_bits(x - back.x, y - back.y);
 }
 
+// Two fp32 numbers to an instruction.
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 floats_of(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 template <int DT>
 __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, const AttendArgs t, const int vec_q, const int vec_out) {
   constexpr int P = DT == SDQ_F32 ? 2 : 1;
@@ -262,7 +288,10 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
     // ---------------------------------------------------------------- converters of values
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
     const int w = warp - 12, tt = threadIdx.x & 127;
-    const int piece = lane & 7, kg = lane >> 3;           // 16 values of d of 8 of this warp's 32 keys
+    // 16 values of d of 8 of this warp's 32 keys.  Neighbouring lanes differ in the keys, and those of odd
+    // pieces store their words in pairs swapped, so that 8 lanes write to 8 different groups of banks (lanes
+    // that differed in d alone would all write to one: 8 times as long, 200 of 880 us).
+    const int piece = lane >> 2, kg = lane & 3, odd = piece & 1;
     const bool has_v = piece * 16 < a.D;
     uint4 vr[8];
     auto load_v = [&](int j) {
@@ -293,8 +322,10 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
             uint32_t h[4][4];   // [value of d][pair of keys]
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
-              const uint32_t u = q == 0 ? vr[e].x : q == 1 ? vr[e].y : q == 2 ? vr[e].z : vr[e].w;
-              const uint32_t v = q == 0 ? vr[e + 1].x : q == 1 ? vr[e + 1].y : q == 2 ? vr[e + 1].z : vr[e + 1].w;
+              auto word = [&](const uint4& x) {   // q ^ odd of x
+                return q < 2 ? ((q ^ odd) ? x.y : x.x) : ((q ^ odd) == 3 ? x.w : x.z);
+              };
+              const uint32_t u = word(vr[e]), v = word(vr[e + 1]);
               const uint32_t x = __byte_perm(u, v, 0x5140) ^ 0x80808080u, y = __byte_perm(u, v, 0x7362) ^ 0x80808080u;
               h[0][e / 2] = bytes_to_half2(x, 0x4140);
               h[1][e / 2] = bytes_to_half2(x, 0x4342);
@@ -303,7 +334,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-              const int d = 16 * piece + 4 * q + i;
+              const int d = 16 * piece + 4 * (q ^ odd) + i;
               st_shared_v4_b32(st + d * 128 + ((chunk ^ (d & 7)) << 4), h[i][0], h[i][1], h[i][2], h[i][3]);
             }
           }
@@ -466,6 +497,59 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
       for (int h = 0; h < 2; h++)
         sees[h] = bk.there[j & 3][grp * 2 + h] & (left >= 32 * h + 32 ? 0xffffffffu : left <= 32 * h ? 0u : (1u << (left - 32 * h)) - 1);
       const bool all = __all_sync(0xffffffffu, (sees[0] & sees[1]) == 0xffffffffu);
+      // One pass with the offset as it stands, while every key is seen and no maximum runs away from it:
+      // the maximum is found beside the weights instead of in front of them.
+      if constexpr (P == 1) {
+        if (all && __all_sync(0xffffffffu, m > -INFINITY)) {
+          const uint64_t f2 = pair_of(factor, factor), e2 = pair_of(e_off, e_off);
+          const ulonglong2* k2 = reinterpret_cast<const ulonglong2*>(ks);
+          const ulonglong2* v2 = reinterpret_cast<const ulonglong2*>(vs);
+          float top[4] = {m, m, m, m};
+          uint64_t sum[4] = {};
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint64_t x[4], k[4], v[4];
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                const ulonglong2 kk = k2[h * 8 + i / 4 + e], vv = v2[h * 8 + i / 4 + e];
+                k[2 * e] = kk.x; k[2 * e + 1] = kk.y;
+                v[2 * e] = vv.x; v[2 * e + 1] = vv.y;
+              }
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                x[e] = mul2(pair_of(__uint_as_float(s[h][i + 2 * e]), __uint_as_float(s[h][i + 2 * e + 1])), k[e]);
+                const float2 y = floats_of(x[e]);
+                top[e] = fmaxf(top[e], fmaxf(y.x, y.y));
+              }
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const float2 y = floats_of(fma2(x[e], f2, e2));
+                x[e] = pair_of(exp2_fast(y.x), exp2_fast(y.y));
+              }
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                sum[e] = add2(sum[e], x[e]);
+                const float2 y = floats_of(mul2(x[e], v[e]));
+                w[i / 2 + e] = half2_bits(y.x, y.y);
+              }
+            }
+            tmem_st_32x16(s_col + 32 * h, w);   // over scores that the registers still hold
+          }
+          const float bm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          if (!__any_sync(0xffffffffu, (bm - m) * factor > kStepUp)) {
+            const float2 y = floats_of(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+            l += y.x + y.y;
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(bk.pready[slot][grp]));
+            continue;
+          }
+        }
+      }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // independent chains
 #pragma unroll
       for (int h = 0; h < 2; h++) {
