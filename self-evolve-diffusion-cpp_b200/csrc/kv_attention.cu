@@ -82,13 +82,13 @@ __global__ void __launch_bounds__(kBlock, 2) kv_attend_few(const KvArgs a, const
   __shared__ float2 block_ml[R];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
-  const int rank = blockIdx.x % ck, kh = blockIdx.y;
+  const int rank = blockIdx.x % ck, kh = blockIdx.x / ck % a.heads;
   const int group = t.heads / a.heads;
 
   allow_dependent_launch();
   wait_prior_grids();
   Tile tile;
-  if (!find_tile(a, group, R, blockIdx.x / ck, &tile)) return;   // the same in all blocks of a cluster
+  if (!find_tile(a, group, R, blockIdx.x / ck / a.heads, &tile)) return;   // the same in all blocks of a cluster
   // keys that the tile's last token sees
   const int last_token = (tile.first_row + tile.rows - 1) / group;
   const int last_pos = t.causal ? (int)max((int64_t)-1, (int64_t)table_at(a.kv_len, tile.b) - tile.n + last_token) : INT_MAX;
@@ -503,7 +503,7 @@ cudaError_t launch_few(const KvArgs& a, const AttendArgs& t, int vec, cudaStream
   }();
   if (set != cudaSuccess) return set;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * ck), (unsigned)a.heads);
+  cfg.gridDim = dim3((unsigned)(tiles * a.heads * ck));
   cfg.blockDim = dim3(kBlock);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = s;

@@ -44,8 +44,8 @@ constexpr int kRowsT = 128;        // rows of a tile
 constexpr int kKeys = 128;         // keys of a block
 constexpr int kPlane = kKeys * 128 * 2;        // 32 KiB: a block's keys or values in fp16
 constexpr int kThreadsT = 640;
-// registers of a thread: 640 threads are launched with 96 each; 256 * 144 + 256 * 72 + 128 * 40 = 60416 of 61440
-constexpr int kRegsSoftmax = 144, kRegsConvert = 72, kRegsIssue = 40;
+// registers of a thread: 640 threads are launched with 96 each; 256 * 136 + 256 * 80 + 128 * 40 = 60416 of 61440
+constexpr int kRegsSoftmax = 136, kRegsConvert = 80, kRegsIssue = 40;
 constexpr int kDrain = 4;          // blocks between two drains of O (fp32 queries)
 constexpr uint32_t kColQhi = 0, kColQlo = 64, kColS = 256;
 __host__ __device__ constexpr uint32_t kColO(int planes, int grp) { return planes == 2 ? 128u : 128u * grp; }
@@ -148,12 +148,11 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
   Book& bk = *reinterpret_cast<Book*>(smem + 4 * kPlane + (P == 2 ? 128 * kRowsT * 4 : kPlane));
   volatile int* abort_flag = &bk.abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kh = blockIdx.y, group = t.heads / a.heads;
+  const int kh = blockIdx.x % a.heads, group = t.heads / a.heads;
 
   wait_prior_grids();
   Tile tile;
-  // the last tiles of a causal sequence see the most keys: they go first
-  if (!find_tile(a, group, kRowsT, (int)(gridDim.x - 1 - blockIdx.x), &tile)) return;
+  if (!find_tile(a, group, kRowsT, blockIdx.x / a.heads, &tile)) return;
   const int last_token = (tile.first_row + tile.rows - 1) / group;
   const int last_pos = t.causal ? (int)max((int64_t)-1, (int64_t)table_at(a.kv_len, tile.b) - tile.n + last_token) : INT_MAX;
   const int keys = max(0, t.causal ? (last_pos < tile.len ? last_pos + 1 : tile.len) : tile.len);
@@ -744,7 +743,7 @@ cudaError_t launch_typed(const KvArgs& a, const AttendArgs& t, cudaStream_t s) {
   const int64_t tiles = (int64_t)a.rows * group / kRowsT + a.batch;
   const int vec_q = (reinterpret_cast<uintptr_t>(t.q) & 15) == 0 && t.ldq * size % 16 == 0;
   const int vec_out = (reinterpret_cast<uintptr_t>(t.out) & 15) == 0 && t.ldo * size % 16 == 0;
-  return launch_overlapped(kv_attend_many<DT>, dim3((unsigned)tiles, (unsigned)a.heads), dim3(kThreadsT), kSmemMany<P>, s, a, t, vec_q, vec_out);
+  return launch_overlapped(kv_attend_many<DT>, dim3((unsigned)(tiles * a.heads)), dim3(kThreadsT), kSmemMany<P>, s, a, t, vec_q, vec_out);
 }
 
 }  // namespace

@@ -91,37 +91,78 @@ __host__ __device__ __forceinline__ int pool_row_of(const KvArgs& a, int row) {
 }
 
 // Row tiles.  The rows of a sequence and one cache head are its new tokens times the `group` query heads
-// that share the head, row = token * group + head; a tile takes T of them.  The tiles of all sequences
-// are numbered without a table: sequence b's begin at row_start[b] * group / T + b, which leaves room for
-// a ragged last one (ceil(n / T) <= floor((s + n) / T) - floor(s / T) + 1); a number that is no tile ends
-// at once.
+// that share the head, row = token * group + head; a tile takes T of them.  Tiles are numbered from the
+// longest sequence down, and inside one from its last rows (which see the most keys) back: blocks run in
+// about that order, so the GPU ends on short pieces.  That takes comparing all sequences with all, which
+// pays up to 64 of them; beyond, sequence b's numbers begin at row_start[b] * group / T + b, which leaves
+// room for a ragged last tile (ceil(n / T) <= floor((s + n) / T) - floor(s / T) + 1), and a number that is no
+// tile ends at once.  Called by whole warps.
 struct Tile {
   int b, first_row, rows;   // sequence; first (token, head) row; how many
   int first, n, len;        // first row of the call, new tokens, keys of the sequence
 };
 __device__ __forceinline__ bool find_tile(const KvArgs& a, int group, int T, int id, Tile* t) {
-  // the last b whose tiles begin at or before id: their first numbers do not decrease, 32 at a time
   const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    bool at_or_before = false;
-    if (b0 + lane < a.batch) {
-      int f, l;
-      seq_rows(a, b0 + lane, f, l);
-      at_or_before = (int64_t)f * group / T + b0 + lane <= id;
+  int in_seq;   // number inside the sequence
+  if (a.batch <= 64) {
+    int len[2], tiles[2], before[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int b = lane + 32 * i;
+      len[i] = -1;
+      tiles[i] = 0;
+      if (b < a.batch) {
+        int f, l;
+        seq_rows(a, b, f, l);
+        len[i] = max(0, table_at(a.kv_len, b));
+        tiles[i] = ((l - f) * group + T - 1) / T;
+      }
     }
-    const uint32_t all = __ballot_sync(0xffffffffu, at_or_before);
-    before += __popc(all);
-    if (all != 0xffffffffu) break;
+    for (int j = 0; j < a.batch; j++) {
+      const int lj = __shfl_sync(0xffffffffu, j < 32 ? len[0] : len[1], j & 31), tj = __shfl_sync(0xffffffffu, j < 32 ? tiles[0] : tiles[1], j & 31);
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+        if (lj > len[i] || (lj == len[i] && j < lane + 32 * i)) before[i] += tj;
+    }
+    int b = -1, at = 0;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const uint32_t it = __ballot_sync(0xffffffffu, id >= before[i] && id < before[i] + tiles[i]);
+      if (it) {
+        const int src = __ffs(it) - 1;
+        b = src + 32 * i;
+        at = __shfl_sync(0xffffffffu, before[i] + tiles[i] - 1, src);
+      }
+    }
+    if (b < 0) return false;
+    t->b = b;
+    in_seq = at - id;
+  } else {
+    // the last b whose tiles begin at or before id: their first numbers do not decrease, 32 at a time
+    int before = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+      bool at_or_before = false;
+      if (b0 + lane < a.batch) {
+        int f, l;
+        seq_rows(a, b0 + lane, f, l);
+        at_or_before = (int64_t)f * group / T + b0 + lane <= id;
+      }
+      const uint32_t all = __ballot_sync(0xffffffffu, at_or_before);
+      before += __popc(all);
+      if (all != 0xffffffffu) break;
+    }
+    if (before == 0) return false;
+    t->b = before - 1;
+    int f, l;
+    seq_rows(a, t->b, f, l);
+    in_seq = id - (int)((int64_t)f * group / T + t->b);
   }
-  if (before == 0) return false;
-  t->b = before - 1;
   int last;
   seq_rows(a, t->b, t->first, last);
   t->n = last - t->first;
-  t->first_row = (id - (int)((int64_t)t->first * group / T + t->b)) * T;
+  t->first_row = in_seq * T;
   t->rows = min(T, t->n * group - t->first_row);
-  if (t->rows <= 0 || t->first_row < 0) return false;   // (below zero only where row_start decreases)
+  if (t->rows <= 0 || in_seq < 0) return false;   // (below zero only where row_start decreases)
   const int64_t most = (int64_t)a.max_pages * a.page_size;
   t->len = (int)max((int64_t)0, min((int64_t)table_at(a.kv_len, t->b), most));
   return true;

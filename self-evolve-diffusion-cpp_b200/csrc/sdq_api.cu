@@ -942,6 +942,7 @@ int sdq_kv_attention(const sdq_kv_cache* cache, const sdq_kv_seqs* seqs, const v
     if (heads <= 0 || heads % a.heads != 0 || heads > 65535) return invalid(kName, "heads must be a positive multiple of the cache's heads");
     if (!(scale > 0.0f) || scale > 1e30f) return invalid(kName, "scale must be positive and finite");
     if (rows * (int64_t)heads > (1 << 30)) return invalid(kName, "rows * heads must fit 30 bits");
+    if (a.batch * (int64_t)a.heads > (1 << 26)) return invalid(kName, "sequences * cache heads must fit 26 bits");
     const bool none = rows == 0 || a.batch == 0;
     if (!none && (!q_dev || !out_dev)) return invalid(kName, "null pointer");
     const int64_t width = (int64_t)heads * a.D;

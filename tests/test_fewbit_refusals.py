@@ -129,6 +129,7 @@ def test_kv_calls(lib, pkg):
     refused(lib, a(c, s, P, 0, 0, 4, 2, float("nan"), P, 0, 0, None), "scale")
     refused(lib, a(c, s, P, 0, 0, 4, 2, float("inf"), P, 0, 0, None), "scale")
     refused(lib, a(c, s, P, 0, 0, 1 << 29, 8, 0.1, P, 0, 0, None), "30 bits")
+    refused(lib, a(cache(pkg, heads=64), seqs(pkg, batch=1 << 21), P, 0, 0, 4, 64, 0.1, P, 0, 0, None), "26 bits")
     refused(lib, a(c, s, None, 0, 0, 4, 2, 0.1, P, 0, 0, None), "null pointer")
     refused(lib, a(c, s, P, 0, 100, 4, 2, 0.1, P, 0, 0, None), "stride")
     refused(lib, a(c, s, P, 0, 0, 4, 2, 0.1, P, 100, 0, None), "stride")
