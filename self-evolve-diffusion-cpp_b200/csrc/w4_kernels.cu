@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kBlock) w4_layout_kernel(const uint8_t* __rest
 //
 // Exactness: q is an integer of 4 bits, exact in either 16-bit type.  fp16 and int8 rows enter as fp16
 // and bf16 rows as bf16, as they are; fp32 rows as two fp16 numbers (hi + lo, 22 bits) times a power of
-// two for each row and slice.  int8 sums are whole numbers below 2^24 and exact.
+// two for each row and tile.  int8 sums are whole numbers below 2^24 and exact.
 __device__ __forceinline__ uint32_t lop3_and_or(uint32_t a, uint32_t mask, uint32_t or_) {
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(mask), "r"(or_));   // (a & mask) | or_
@@ -184,7 +184,7 @@ __device__ __forceinline__ float2 scale_pair(const uint8_t* p) {
 // the end of a row tile, and a row tile that crosses warps is summed afterwards.
 struct W4Plan {
   int ck, strips_long, strip, slice, stage, slots;
-  int x, red, part;   // offsets in shared memory, in bytes
+  int x, exp, red, part;   // offsets in shared memory, in bytes
 };
 
 constexpr int kWarps = kBlock / 32;
@@ -224,50 +224,43 @@ __device__ __forceinline__ void fill_x(const W4Args& a, int m0, int rows, int k0
     }
   };
   if constexpr (XT == SDQ_F32) {
-    // largest finite |x| of each row into [2^14, 2^15): fp16 holds it, and lo's last place lies 2^-39
-    // below it
-    const int parts = kWarps / rows, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if ((int)threadIdx.x < rows) row_exp[threadIdx.x] = 0.0f;
-    __syncthreads();
-    const int nv = tiles * 32;
-    if (warp < rows * parts) {
-      const int r = warp % rows, part = warp / rows;
-      float mx = 0.0f;
-#pragma unroll 4
-      for (int v = part * 32 + lane; v < nv; v += 32 * parts) {
-        float f[4];
-        floats4(r, k0 + v * 4, f);
+    // A warp takes one row of one tile, 4 columns to a lane: its largest finite |x| into [2^14, 2^15), where
+    // fp16 holds it, and lo's last place lies 2^-39 below it.
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pairs = rows * tiles;
+    constexpr int U = 4;
+    for (int p0 = warp; p0 < pairs; p0 += kWarps * U) {
+      float f[U][4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) mx = fabsf(f[e]) <= 3.402823466e38f ? fmaxf(mx, fabsf(f[e])) : mx;
-      }
-      mx = warp_max(mx);
-      if (lane == 0) atomicMax(reinterpret_cast<int*>(row_exp) + r, __float_as_int(mx));   // order of positive floats
-    }
-    __syncthreads();
-    if ((int)threadIdx.x < rows) {
-      const float mx = row_exp[threadIdx.x];
-      const int e = max(mx > 0.0f ? ilogbf(mx) - 14 : 0, -126);
-      row_exp[threadIdx.x] = __uint_as_float((uint32_t)(e + 127) << 23);   // 2^e, e in -126..113
-    }
-    __syncthreads();
-    uint2* dst = reinterpret_cast<uint2*>(smem);
-#pragma unroll 2
-    for (int i = threadIdx.x; i < nv * rows; i += kBlock) {
-      const int r = i / nv, v = i - r * nv;
-      float f[4];
-      floats4(r, k0 + v * 4, f);
-      const float inv = __uint_as_float((254u << 23) - __float_as_uint(row_exp[r]));   // 2^-e, exact
-      uint32_t hi[2], lo[2];
+      for (int u = 0; u < U; u++) {
+        const int p = p0 + u * kWarps, tile = p / rows;
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const float p = f[2 * e] * inv, q = f[2 * e + 1] * inv;
-        hi[e] = half2_bits(p, q);
-        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-        lo[e] = half2_bits(isinf(back.x) ? 0.0f : p - back.x, isinf(back.y) ? 0.0f : q - back.y);   // an infinity has no rest
+        for (int e = 0; e < 4; e++) f[u][e] = 0.0f;
+        if (p < pairs) floats4(p - tile * rows, k0 + tile * 128 + lane * 4, f[u]);
       }
-      const int at = ((v >> 3) * 2 * rows + r) * 8 + (v & 7);
-      dst[at] = make_uint2(hi[0], hi[1]);
-      dst[at + rows * 8] = make_uint2(lo[0], lo[1]);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int p = p0 + u * kWarps, tile = p / rows, r = p - tile * rows;
+        float mx = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) mx = fabsf(f[u][e]) <= 3.402823466e38f ? fmaxf(mx, fabsf(f[u][e])) : mx;
+        mx = warp_max(mx);
+        if (p < pairs) {
+          const int e2 = max((int)(__float_as_uint(mx) >> 23) - 127 - 14, -126);   // -126..113
+          const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
+          if (lane == 0) row_exp[tile * kRows + r] = __uint_as_float((uint32_t)(e2 + 127) << 23);
+          uint32_t hi[2], lo[2];
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const float x = f[u][2 * e] * inv, y = f[u][2 * e + 1] * inv;
+            hi[e] = half2_bits(x, y);
+            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+            lo[e] = half2_bits(isinf(back.x) ? 0.0f : x - back.x, isinf(back.y) ? 0.0f : y - back.y);   // an infinity has no rest
+          }
+          uint2* dst = reinterpret_cast<uint2*>(smem) + ((tile * 4 + (lane >> 3)) * 2 * rows + r) * 8 + (lane & 7);
+          dst[0] = make_uint2(hi[0], hi[1]);
+          dst[rows * 8] = make_uint2(lo[0], lo[1]);
+        }
+      }
     }
   } else if constexpr (XT == SDQ_I8) {
     const int nv = tiles * 8;
@@ -320,7 +313,7 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) w4_rows_kernel(const W4A
   constexpr int P = XT == SDQ_F32 ? 2 : 1;
   constexpr int SS = ST == SDQ_F32 ? 4 : 2, kTile = kTileBytes(SS, GROUP), kScalePieces = (kTile - 1024) / 16;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float row_exp[kRows];   // fp32 rows: 2^e of the stage
+  float* row_exp = reinterpret_cast<float*>(smem + p.exp);   // fp32 rows: 2^e of every tile and row
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int rank = blockIdx.x % p.ck, strip = blockIdx.x / p.ck;
@@ -339,6 +332,8 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) w4_rows_kernel(const W4A
 
   allow_dependent_launch();
   bool first = true;
+  __shared__ int first_row[kWarps];   // row tile that each warp's run begins in
+  const int share = threadIdx.x / box, within = threadIdx.x - share * box, shares = kBlock / box;   // of the sums below
   for (int s0 = slice0; s0 < slice1 || first; s0 += p.stage) {   // once at least: a block without columns adds zeros
     const int tiles = max(0, min(p.stage, slice1 - s0));
     const int run = (strip_rows * tiles + kWarps - 1) / kWarps;
@@ -368,12 +363,8 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) w4_rows_kernel(const W4A
     if (first) wait_prior_grids();   // the weights are there from the upload on; x, bias and out belong to the stream
     fill_x<XT>(a, m0, rows, s0 * 128, tiles, vec, smem + p.x, row_exp);
     __syncthreads();
-    float ex[2] = {};
-    if constexpr (P == 2) {
-#pragma unroll
-      for (int j = 0; j < 2; j++) ex[j] = 2 * c + j < rows ? row_exp[2 * c + j] : 0.0f;
-    }
     float y[4] = {}, acc[4];
+    const float2* exb = reinterpret_cast<const float2*>(row_exp) + t0 * (kRows / 2) + c;   // rows 2 c, 2 c + 1
     // lanes of columns that no row of x fills read the last row: what they compute is never stored
     const uint4* x_lane = reinterpret_cast<const uint4*>(smem + p.x) + min(g, rows - 1) * 4 + c;
     const uint4* xb = x_lane + t0 * (4 * P * 4) * rows;
@@ -384,6 +375,11 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) w4_rows_kernel(const W4A
       __syncwarp();   // the scales are other lanes' copies
       const uint8_t* piece = ring + at * kTile;
       const uint4 w0 = *reinterpret_cast<const uint4*>(piece + lane * 16), w1 = *reinterpret_cast<const uint4*>(piece + lane * 16 + 512);
+      float2 ex = make_float2(1.0f, 1.0f);
+      if constexpr (P == 2) {
+        ex = *exb;   // of rows that are none: whatever lies there, for sums that are never stored
+        exb += kRows / 2;
+      }
       const uint32_t words[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
       for (int j = 0; j < 4; j++) {      // 32 columns
@@ -405,7 +401,7 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) w4_rows_kernel(const W4A
           const float2 f = scale_pair<ST>(piece + 1024 + (32 * j / GROUP) * (16 * SS) + g * (2 * SS));
           if constexpr (P == 2) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) acc[e] *= ex[e & 1];
+            for (int e = 0; e < 4; e++) acc[e] *= e & 1 ? ex.y : ex.x;
           }
           y[0] = fmaf(acc[0], f.x, y[0]);
           y[1] = fmaf(acc[1], f.x, y[1]);
@@ -429,26 +425,28 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) w4_rows_kernel(const W4A
         y[0] = y[1] = y[2] = y[3] = 0.0f;
         to_store = tiles;
         xb = x_lane;
+        exb = reinterpret_cast<const float2*>(row_exp) + c;
         slot++;
       }
     }
     copies_wait<0>();
+    if (lane == 0) first_row[warp] = r0;
     __syncthreads();
     // ---- the block's sums: row tile r lies in the warps whose runs touch [r, r + 1) * tiles ----
-    for (int i = threadIdx.x; i < strip_rows * box; i += kBlock) {
-      const int r = i / box, e = i - r * box;
-      float s = first ? 0.0f : part[i];
-      if (tiles > 0) {
-        const int k0 = r * tiles / run, k1 = ((r + 1) * tiles - 1) / run;
-        for (int k = k0; k <= k1; k++) s += red[(k * p.slots + r - k * run / tiles) * box + e];
+    if (share < shares) {
+      for (int r = share; r < strip_rows; r += shares) {
+        float s = first ? 0.0f : part[r * box + within];
+#pragma unroll
+        for (int k = 0; k < kWarps; k++)
+          if (k * run < (r + 1) * tiles && (k + 1) * run > r * tiles) s += red[(k * p.slots + r - first_row[k]) * box + within];
+        part[r * box + within] = s;
       }
-      part[i] = s;
     }
     first = false;
     if (s0 + p.stage < slice1) __syncthreads();   // x and the sums are read before the next stage writes them
   }
-  auto finish = [&](int i, float s) {
-    const int r = i / box, m = (i - r * box) >> 4;
+  auto finish = [&](int r, float s) {   // element `within` of row tile r
+    const int m = within >> 4, i = within;
     const int64_t n = ((int64_t)row0 + r) * 16 + (i & 15);
     if (n >= a.N) return;
     if (XT == SDQ_I8) s *= a.x_scale[m0 + m];
@@ -459,16 +457,19 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) w4_rows_kernel(const W4A
     else if (a.out_dtype == SDQ_BF16) store_dst<SDQ_BF16>(a.out, o, s);
     else store_dst<SDQ_F16>(a.out, o, s);
   };
-  const int count = strip_rows * box;
   if (p.ck == 1) {
-    for (int i = threadIdx.x; i < count; i += kBlock) finish(i, part[i]);   // each thread its own sums
+    if (share < shares)
+      for (int r = share; r < strip_rows; r += shares) finish(r, part[r * box + within]);   // each thread its own sums
   } else {
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    for (int i = rank * kBlock + threadIdx.x; i < count; i += kBlock * p.ck) {
-      float s = 0.0f;
-      for (int r = 0; r < p.ck; r++) s += cluster.map_shared_rank(part, r)[i];
-      finish(i, s);
+    if (share < shares) {
+      for (int r = rank * shares + share; r < strip_rows; r += shares * p.ck) {
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = k < p.ck ? cluster.map_shared_rank(part, k)[r * box + within] : 0.0f;
+        finish(r, ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])));
+      }
     }
     cluster.sync();   // nobody leaves while its sums may be read
   }
@@ -493,7 +494,8 @@ bool w4_cut(int64_t N, int64_t K, int rows, int planes, int ring, int ck, int wa
     // tiles, which is no more than strip / warps + 2 for any t
     p->slots = p->strip / kWarps + 2;
     p->x = ring * kWarps;
-    p->red = p->x + p->stage * tile_bytes;
+    p->exp = p->x + p->stage * tile_bytes;
+    p->red = p->exp + (planes == 2 ? p->stage * kRows * 4 : 0);
     p->part = p->red + kWarps * p->slots * rows * 64;
     *smem = p->part + p->strip * rows * 64;
     if (*smem <= kSmemMost) return true;
