@@ -227,39 +227,51 @@ __device__ __forceinline__ void fill_x(const W4Args& a, int m0, int rows, int k0
     // A warp takes one row of one tile, 4 columns to a lane: its largest finite |x| into [2^14, 2^15), where
     // fp16 holds it, and lo's last place lies 2^-39 below it.
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pairs = rows * tiles;
-    constexpr int U = 4;
+    const uint32_t by_rows = (65536u + rows - 1) / rows;   // p / rows by a product: right while p * (rows - 1) < 2^16,
+                                                           // and no stage has 2^13 pairs (shared memory holds 512 B of each)
+    constexpr int U = 7;
     for (int p0 = warp; p0 < pairs; p0 += kWarps * U) {
       float f[U][4];
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const int p = p0 + u * kWarps, tile = p / rows;
+        const int p = p0 + u * kWarps, tile = (int)((uint32_t)p * by_rows >> 16);
 #pragma unroll
         for (int e = 0; e < 4; e++) f[u][e] = 0.0f;
         if (p < pairs) floats4(p - tile * rows, k0 + tile * 128 + lane * 4, f[u]);
       }
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const int p = p0 + u * kWarps, tile = p / rows, r = p - tile * rows;
-        float mx = 0.0f;
+        const int p = p0 + u * kWarps, tile = (int)((uint32_t)p * by_rows >> 16), r = p - tile * rows;
+        if (p >= pairs) break;
+        uint32_t mag[4], mx;   // |x| as bits, which order like the numbers; infinities and NaN come last
 #pragma unroll
-        for (int e = 0; e < 4; e++) mx = fabsf(f[u][e]) <= 3.402823466e38f ? fmaxf(mx, fabsf(f[u][e])) : mx;
-        mx = warp_max(mx);
-        if (p < pairs) {
-          const int e2 = max((int)(__float_as_uint(mx) >> 23) - 127 - 14, -126);   // -126..113
-          const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
-          if (lane == 0) row_exp[tile * kRows + r] = __uint_as_float((uint32_t)(e2 + 127) << 23);
-          uint32_t hi[2], lo[2];
+        for (int e = 0; e < 4; e++) mag[e] = __float_as_uint(f[u][e]) & 0x7fffffffu;
+        mx = __reduce_max_sync(0xffffffffu, max(max(mag[0], mag[1]), max(mag[2], mag[3])));
+        const bool finite = mx < 0x7f800000u;
+        if (!finite) {
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const float x = f[u][2 * e] * inv, y = f[u][2 * e + 1] * inv;
-            hi[e] = half2_bits(x, y);
-            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-            lo[e] = half2_bits(isinf(back.x) ? 0.0f : x - back.x, isinf(back.y) ? 0.0f : y - back.y);   // an infinity has no rest
-          }
-          uint2* dst = reinterpret_cast<uint2*>(smem) + ((tile * 4 + (lane >> 3)) * 2 * rows + r) * 8 + (lane & 7);
-          dst[0] = make_uint2(hi[0], hi[1]);
-          dst[rows * 8] = make_uint2(lo[0], lo[1]);
+          for (int e = 0; e < 4; e++) mag[e] = mag[e] < 0x7f800000u ? mag[e] : 0u;
+          mx = __reduce_max_sync(0xffffffffu, max(max(mag[0], mag[1]), max(mag[2], mag[3])));
         }
+        const int e2 = max((int)(mx >> 23) - 127 - 14, -126);   // -126..113
+        const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
+        if (lane == 0) row_exp[tile * kRows + r] = __uint_as_float((uint32_t)(e2 + 127) << 23);
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const float x = f[u][2 * e] * inv, y = f[u][2 * e + 1] * inv;
+          hi[e] = half2_bits(x, y);
+          float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+          float rx = x - back.x, ry = y - back.y;
+          if (!finite) {   // an infinity has no rest
+            rx = isinf(back.x) ? 0.0f : rx;
+            ry = isinf(back.y) ? 0.0f : ry;
+          }
+          lo[e] = half2_bits(rx, ry);
+        }
+        uint2* dst = reinterpret_cast<uint2*>(smem) + ((tile * 4 + (lane >> 3)) * 2 * rows + r) * 8 + (lane & 7);
+        dst[0] = make_uint2(hi[0], hi[1]);
+        dst[rows * 8] = make_uint2(lo[0], lo[1]);
       }
     }
   } else if constexpr (XT == SDQ_I8) {
