@@ -485,16 +485,21 @@ __global__ void __launch_bounds__(kBlock, 2) kv_attend_few(const KvArgs a, const
   cluster.sync();   // nobody leaves while its sums may be read
 }
 
+// As many blocks to a sequence and cache head as fill the GPU at two to an SM, and leave a warp a step.
+// One sequence of 32k keys, 8 heads: 247 us with 1 block, 68 with 4, 30.8 with 16; 64 of 4k: 86 with 1,
+// 94 with 2, 118 with 4.
+int split_few(const KvArgs& a) {
+  int ck = 1;
+  const int64_t work = (int64_t)a.batch * a.heads, most = (int64_t)a.max_pages * a.page_size;
+  while (ck < 16 && work * ck * 2 <= 296 && most >= (int64_t)ck * 2 * kWarps * kStep) ck *= 2;
+  return ck;
+}
+
 template <int DT, int NJ, int NT>
 cudaError_t launch_few(const KvArgs& a, const AttendArgs& t, int vec, cudaStream_t s) {
   const int group = t.heads / a.heads;
   const int64_t tiles = (int64_t)a.rows * group / (8 * NT) + a.batch;   // with numbers that are no tile, see Tile
-  // As many blocks to a sequence and cache head as fill the GPU at two to an SM, and leave a warp a step.
-  // One sequence of 32k keys, 8 heads: 247 us with 1 block, 68 with 4, 30.8 with 16; 64 of 4k: 86 with 1,
-  // 94 with 2, 118 with 4.
-  int ck = 1;
-  const int64_t work = (int64_t)a.batch * a.heads, most = (int64_t)a.max_pages * a.page_size;
-  while (ck < 16 && work * ck * 2 <= 296 && most >= (int64_t)ck * 2 * kWarps * kStep) ck *= 2;
+  const int ck = split_few(a);
   constexpr int kSmem = kWarps * kDepth * Stage<NJ>::kBytes > kWarps * 8 * NT * 64 * NJ * 4 ? kWarps * kDepth * Stage<NJ>::kBytes
                                                                                          : kWarps * 8 * NT * 64 * NJ * 4;
   static const cudaError_t set = [] {
@@ -531,7 +536,13 @@ cudaError_t launch_typed(const KvArgs& a, const AttendArgs& t, cudaStream_t s) {
 
 cudaError_t launch_kv_attention(const KvArgs& a, const AttendArgs& t, int dtype, cudaStream_t s) {
   count_launch();
-  if ((int64_t)a.rows * (t.heads / a.heads) > (int64_t)32 * a.batch) return launch_kv_attend_many(a, t, dtype, s);
+  // Tiles of 128 rows on tcgen05 from 33 rows to a sequence (a row: a token and a query head) on the average,
+  // once the blocks here would go round more than 1.3 times.  bf16, here / there, us: 64 sequences of 2k keys,
+  // 8 heads: 32 rows 131 / 157, 48 rows 176 / 169, 128 rows 432 / 230; one of 32k, 8 heads: 48 rows 79 / 92
+  // (384 blocks), 64 rows 115 / 91 (512); one of 32k, 1 head: 128 rows 40 / 81, 256 rows 69 / 82 (256 blocks),
+  // 512 rows 112 / 83; one of 2k, 4 heads, the rule's worst: 128 rows 37 / 26 (256 blocks).
+  const int64_t mean = ((int64_t)a.rows * (t.heads / a.heads) + a.batch - 1) / a.batch;
+  if (mean > 32 && (mean + 15) / 16 * a.batch * a.heads * split_few(a) > 384) return launch_kv_attend_many(a, t, dtype, s);
   if (dtype == SDQ_F32) return launch_typed<SDQ_F32>(a, t, s);
   if (dtype == SDQ_BF16) return launch_typed<SDQ_BF16>(a, t, s);
   return launch_typed<SDQ_F16>(a, t, s);

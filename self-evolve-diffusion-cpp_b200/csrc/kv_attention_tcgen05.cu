@@ -23,9 +23,10 @@
 //
 // Softmax in one sweep with a running offset m of each row: p = 2^6 2^(s - m); the offset moves, and O and
 // the row's sum are scaled down, only when a block's maximum exceeds it by more than 9 log2 units, so a
-// weight stays below 2^15 and inside fp16, whose grid ends at 2^-31 of the weight at the offset.  (With 4
-// units a fifth of the blocks had some row of a warp that moved, and scaling O costs as much as a block's
-// exponentials.)  With fp32 queries O is taken out of tensor memory every kDrain blocks and added up in
+// weight stays below 2^15 and inside fp16, whose grid ends at 2^-30 of the weight at the offset and of the
+// largest v scale: each key's share is off by 2^-23 of that scale at most, however small its own is.  A larger
+// power than 2^6 would move that down and the offset more often, which scales O and costs as much as a
+// block's exponentials: fp32, 2 x 1000 rows, 8000 keys, 24 heads: 381 us with 2^6, 422 with 2^8, 490 with 2^10.  With fp32 queries O is taken out of tensor memory every kDrain blocks and added up in
 // shared memory in fp32: the tensor core's accumulator truncates, and over thousands of keys that would be
 // the largest error there is (1e-5 of the result at 4k keys).
 //
@@ -33,8 +34,12 @@
 // issue) with the conversion beside it (~450); the MMAs need 512..1024 per product.
 //
 // Every mbarrier wait is bounded like the GEMM kernels'.
+#include <cooperative_groups.h>
+
 #include "kv_common.cuh"
 #include "tc_common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace sdq {
 namespace {
@@ -59,11 +64,14 @@ struct Book {
   int rows[2][4][kKeys];              // pool rows, as the converters of keys and of values looked them up
   float meet[2][2][kRowsT];           // what the two threads of a row tell each other
   float sum[2][kRowsT], off[2][kRowsT];   // sums and offsets of the two halves
+  float all_sum[kRowsT], all_off[kRowsT], factor[kRowsT];   // of this block's share of the keys, for the cluster
   uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pready[2][2], pvdone[2][2], scales[4], qready, lready, ofull, pair[4];
   uint32_t v_top;
   uint32_t tmem;
   int abort;
 };
+constexpr int kJoinRow = 132;      // floats from row to row of a block's results: 8 rows side by side fill the banks once
+static_assert(kRowsT * kJoinRow * 4 <= 4 * kPlane, "the results lie over the operand tiles");
 constexpr int kSlack = 1024;       // to bring the dynamic base to a 1024-byte boundary
 template <int P>
 constexpr int kSmemMany = 4 * kPlane + (P == 2 ? 128 * kRowsT * 4 : kPlane) + (int)sizeof(Book) + kSlack;
@@ -135,8 +143,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-template <int DT>
-__global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, const AttendArgs t, const int vec_q, const int vec_out) {
+// SPLIT: clusters of `blocks` CTAs share a tile's keys; without, `blocks` is 1 and known to the compiler
+// (which otherwise spills: 3 to 6 % of the time).
+template <int DT, bool SPLIT>
+__global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, const AttendArgs t, const int blocks, const int vec_q, const int vec_out) {
+  const int ck = SPLIT ? blocks : 1;
   constexpr int P = DT == SDQ_F32 ? 2 : 1;
   constexpr int EPV = Vec<DT>::EPV;
   extern __shared__ uint8_t smem_raw[];
@@ -145,20 +156,25 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
   const uint32_t smem_v = base + 2 * kPlane;
   const uint32_t smem_q = base + 4 * kPlane;                      // 16-bit queries: q as operand tile
   float* drained = reinterpret_cast<float*>(smem + 4 * kPlane);   // fp32 queries: [d][row], O so far
+  float* joined = reinterpret_cast<float*>(smem);                 // [row][d], this block's result for its cluster
   Book& bk = *reinterpret_cast<Book*>(smem + 4 * kPlane + (P == 2 ? 128 * kRowsT * 4 : kPlane));
   volatile int* abort_flag = &bk.abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kh = blockIdx.x % a.heads, group = t.heads / a.heads;
+  const int rank = SPLIT ? blockIdx.x % ck : 0, kh = blockIdx.x / ck % a.heads, group = t.heads / a.heads;
 
   wait_prior_grids();
   Tile tile;
-  if (!find_tile(a, group, kRowsT, blockIdx.x / a.heads, &tile)) return;
+  if (!find_tile(a, group, kRowsT, blockIdx.x / ck / a.heads, &tile)) return;
   const int last_token = (tile.first_row + tile.rows - 1) / group;
   const int last_pos = t.causal ? (int)max((int64_t)-1, (int64_t)table_at(a.kv_len, tile.b) - tile.n + last_token) : INT_MAX;
-  const int keys = max(0, t.causal ? (last_pos < tile.len ? last_pos + 1 : tile.len) : tile.len);
-  const int nblk = (keys + kKeys - 1) / kKeys;
+  const int all_keys = max(0, t.causal ? (last_pos < tile.len ? last_pos + 1 : tile.len) : tile.len);
+  // the blocks of a cluster take runs of whole key blocks; below, keys count from this block's first one
+  const int per = (int)((((uint32_t)all_keys + kKeys - 1) / kKeys + ck - 1) / ck);
+  const int key0 = !SPLIT ? 0 : (int)min((int64_t)all_keys, (int64_t)rank * per * kKeys);
+  const int keys = SPLIT ? (int)min((int64_t)(all_keys - key0), (int64_t)per * kKeys) : all_keys;
+  const int nblk = (int)(((uint32_t)keys + kKeys - 1) / kKeys);
   auto place = [&](int p) {   // pool row of key p for this cache head, -1: absent
-    const int r = p < keys ? pool_row(a, tile.b, p) : -1;
+    const int r = p < keys ? pool_row(a, tile.b, key0 + p) : -1;
     return r < 0 ? -1 : r + kh * a.page_size;
   };
   auto bar = [&](const uint64_t& b) { return smem_u32(&b); };
@@ -411,7 +427,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const int rr = tile.first_row + r, token = rr / group, head = kh * group + (rr - token * group);
     const bool live = r < tile.rows;
-    const int seen = !live ? 0 : t.causal ? max(0, last_pos - last_token + token + 1) : INT_MAX;   // keys in front of the row's end
+    const int seen = !live ? 0 : t.causal ? max(0, last_pos - last_token + token + 1 - key0) : INT_MAX;   // keys in front of the row's end
     uint32_t pair_ph = 0;
     bool ok = true;
     auto pair_sync = [&]() {   // this warp and the one with the other half of the same rows
@@ -666,8 +682,8 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
     if (ok) {
       tc_fence_after();
       float f[2] = {1.0f, 1.0f};   // brings the halves to one offset
+      const float top = fmaxf(bk.off[0][r], bk.off[1][r]);
       if constexpr (P == 1) {
-        const float top = fmaxf(bk.off[0][r], bk.off[1][r]);
 #pragma unroll
         for (int h = 0; h < 2; h++)
           if (top != -INFINITY) f[h] = exp2_fast((bk.off[h][r] - top) * factor);
@@ -675,6 +691,11 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
       l = bk.sum[0][r] * f[0] + bk.sum[1][r] * f[1];
       const float inv = l != 0.0f ? (1.0f / l) * pow2f(ev) : 0.0f;   // a row that sees no key is zero
       const int64_t at = (int64_t)(tile.first + token) * t.ldo + (int64_t)head * a.D;
+      if (SPLIT && grp == 0) {
+        bk.all_sum[r] = l;
+        bk.all_off[r] = top;
+        bk.factor[r] = factor;
+      }
 #pragma unroll 1
       for (int c = 2 * grp; c < 2 * grp + 2; c++) {
         if (c * 32 >= a.D) break;
@@ -702,7 +723,11 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
 #pragma unroll
           for (int i = 0; i < 32; i++) o[i] = 0.0f;
         }
-        if (live) {
+        if constexpr (SPLIT) {   // over the operand tiles, whose products are done
+          float4* dst = reinterpret_cast<float4*>(joined + r * kJoinRow + c * 32);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) dst[i / 4] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        } else if (live) {
 #pragma unroll
           for (int i = 0; i < 32; i += EPV) {
             if (c * 32 + i >= a.D) break;
@@ -720,6 +745,48 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
       }
       tc_fence_before();
     }
+  }
+
+  // ---- the blocks of a cluster: each has softmax(its keys) V and the sum and offset behind it ----
+  if constexpr (SPLIT) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    if (warp < 8 && !*abort_flag) {
+      const int share = kRowsT / ck;   // rows that this block finishes, 16 threads to a row, 8 values of d to a thread
+      for (int it = threadIdx.x; it < share * 16; it += 256) {
+        const int r = rank * share + (it >> 4), d0 = (it & 15) * 8;
+        if (r >= tile.rows || d0 >= a.D) continue;
+        const float factor = bk.factor[r];
+        float top = -INFINITY, l = 0.0f, o[8] = {};
+        for (int k = 0; k < ck; k++) top = fmaxf(top, cluster.map_shared_rank(&bk.all_off[r], k)[0]);
+        for (int k = 0; k < ck; k++) {
+          const float off = cluster.map_shared_rank(&bk.all_off[r], k)[0];
+          const float w = cluster.map_shared_rank(&bk.all_sum[r], k)[0] * (top != -INFINITY ? exp2_fast((off - top) * factor) : 1.0f);
+          const float4* src = reinterpret_cast<const float4*>(cluster.map_shared_rank(joined, k) + r * kJoinRow + d0);
+          const float4 x = src[0], y = src[1];
+          const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+          l += w;
+#pragma unroll
+          for (int e = 0; e < 8; e++) o[e] = fmaf(w, v[e], o[e]);
+        }
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;   // a row that sees no key is zero
+        const int rr = tile.first_row + r, token = rr / group;
+        const int64_t at = (int64_t)(tile.first + token) * t.ldo + (int64_t)(kh * group + (rr - token * group)) * a.D + d0;
+#pragma unroll
+        for (int i = 0; i < 8; i += EPV) {
+          float y[EPV];
+#pragma unroll
+          for (int e = 0; e < EPV; e++) y[e] = o[i + e] * inv;
+          if (vec_out) {
+            *reinterpret_cast<uint4*>(static_cast<char*>(t.out) + (at + i) * (16 / EPV)) = Vec<DT>::pack(y);
+          } else {
+#pragma unroll
+            for (int e = 0; e < EPV; e++) store_dst<DT>(t.out, at + i + e, y[e]);
+          }
+        }
+      }
+    }
+    cluster.sync();   // nobody leaves while its results may be read
   }
 
   // -------------------------------------------------------------------- common exit
@@ -743,15 +810,43 @@ cudaError_t launch_typed(const KvArgs& a, const AttendArgs& t, cudaStream_t s) {
   const int64_t tiles = (int64_t)a.rows * group / kRowsT + a.batch;
   const int vec_q = (reinterpret_cast<uintptr_t>(t.q) & 15) == 0 && t.ldq * size % 16 == 0;
   const int vec_out = (reinterpret_cast<uintptr_t>(t.out) & 15) == 0 && t.ldo * size % 16 == 0;
-  return launch_overlapped(kv_attend_many<DT>, dim3((unsigned)(tiles * a.heads)), dim3(kThreadsT), kSmemMany<P>, s, a, t, vec_q, vec_out);
+  int ck = 1;
+  const int64_t mean = ((int64_t)a.rows * group + a.batch - 1) / a.batch, work = (mean + kRowsT - 1) / kRowsT * a.batch * a.heads;
+  const int64_t most = (int64_t)a.max_pages * a.page_size;
+  // Clusters share a tile's keys while all of them run at a time (one CTA to an SM), and a CTA has two blocks
+  // of keys.  One sequence of 32k keys, 8 heads, 64 rows: 528 us without, 152 with 4, 90 with 8; 256 rows, 16
+  // clusters of 8, which do not fit: 160, 140 with 4.
+  static const int kFit[3] = {74, 34, 14};
+  for (int i = 0; i < 3 && work <= kFit[i] && most >= (int64_t)ck * 2 * 2 * kKeys; i++) ck *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * a.heads * ck));
+  cfg.blockDim = dim3(kThreadsT);
+  cfg.dynamicSmemBytes = kSmemMany<P>;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim = {(unsigned)ck, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = ck > 1 ? 2 : 1;
+  return ck > 1 ? cudaLaunchKernelEx(&cfg, kv_attend_many<DT, true>, a, t, ck, vec_q, vec_out)
+                : cudaLaunchKernelEx(&cfg, kv_attend_many<DT, false>, a, t, ck, vec_q, vec_out);
+}
+
+template <int DT>
+cudaError_t allow_smem() {
+  constexpr int kSmem = kSmemMany<DT == SDQ_F32 ? 2 : 1>;
+  const cudaError_t e = cudaFuncSetAttribute(kv_attend_many<DT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  return e != cudaSuccess ? e : cudaFuncSetAttribute(kv_attend_many<DT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
 }
 
 }  // namespace
 
 int kv_attend_many_setup(std::string* why) {
-  cudaError_t e = cudaFuncSetAttribute(kv_attend_many<SDQ_F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMany<2>);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kv_attend_many<SDQ_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMany<1>);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kv_attend_many<SDQ_F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMany<1>);
+  cudaError_t e = allow_smem<SDQ_F32>();
+  if (e == cudaSuccess) e = allow_smem<SDQ_BF16>();
+  if (e == cudaSuccess) e = allow_smem<SDQ_F16>();
   if (e != cudaSuccess) {
     if (why) *why = std::string("cache attention set-up: ") + cudaGetErrorString(e);
     return SDQ_ERR_CUDA;

@@ -80,16 +80,16 @@ class Pool:
 
 
 def attention64(pool, q, heads, scale, causal, b):
-    """(out, bound on |out - exact| that the arithmetic of the score and of the weights allows, sum p |v|)
-    of the rows of sequence b; q float64 [rows, heads, dim]."""
+    """Of the rows of sequence b: the output, sum p |v|, the largest sum |q k| of a score (each [rows, heads, ..]) and
+    the sum of exp(score - largest score); q float64 [rows, heads, dim]."""
     group = heads // pool.heads
     k, v = pool.dense(b, "k"), pool.dense(b, "v")
     first, n, L = int(pool.starts[b]), pool.new[b], pool.keys[b]
     out = np.zeros((n, heads, pool.dim))
     mag = np.zeros_like(out)
-    smag = np.zeros((n, heads))
+    smag, total = np.zeros((n, heads)), np.ones((n, heads))
     if L == 0 or n == 0:
-        return out, mag, smag
+        return out, mag, smag, total
     qb = q[first:first + n]
     for h in range(heads):
         kk, vv = k[:, h // group], v[:, h // group]
@@ -105,11 +105,12 @@ def attention64(pool, q, heads, scale, causal, b):
         p = np.where(seen, np.exp(s - np.where(np.isfinite(m), m, 0)), 0.0)
         l = p.sum(1, keepdims=True)
         p = np.where(l > 0, p / np.where(l > 0, l, 1), 0.0)
+        total[:, h] = np.maximum(l[:, 0], 1)
         out[:, h], mag[:, h], smag[:, h] = p @ vv, p @ np.abs(vv), np.max(np.where(seen, a, 0), 1)
-    return out, mag, smag
+    return out, mag, smag, total
 
 
-def attention_tolerance(name, pool, b, out, mag, smag):
+def attention_tolerance(name, pool, b, heads, out, mag, smag, total):
     """What the kernel's roundings add up to at most, element by element.
 
     A score is off by its two factors' roundings (q in 11 bits of a power of two, or 22 with fp32; the
@@ -121,13 +122,18 @@ def attention_tolerance(name, pool, b, out, mag, smag):
     sum and in the output.  Then the output's own rounding: half a step relative to the value, and for
     fp16, whose numbers below 2^-14 lie on a grid of 2^-24, at least half of that grid (2^-25).
 
-    Weights are fp16 numbers in units that put the largest v_scale of the sequence into [2^14, 2^15), and
-    fp16's grid ends at 2^-24: a weight is off by 2^-25 units, 2^-39 of that scale, however small it is.
-    Times codes of at most 2^7, for every key: keys * 2^-32 * max v_scale (the sum of the p is >= 1)."""
+    Weights are fp16 numbers, and fp16's grid ends at 2^-24: a weight is off by 2^-25 units, however small it
+    is.  With up to 32 rows to a sequence the units put the largest v_scale of the sequence into [2^14, 2^15):
+    2^-39 of that scale, times codes of at most 2^7, for every key: keys * 2^-32 * max v_scale, over the sum
+    of the p, which is 1 or more.  Tiles of 128 rows leave room above the running offset: their units are
+    2^ev / 2^6 with 2^ev <= 2 max v_scale, so a weight is off by 2^-25 * 2^-5 = 2^-30 of that scale, and the
+    keys by keys * 2^-23 * max v_scale over the sum of the p."""
     keys = pool.keys[b]
     pg, off = pool.places(b)
     vmax = float(pool.vs.cpu().numpy()[pg, :, off].max()) if keys else 0.0
     score = smag * (2.0 ** -22 + 16 * 2.0 ** -23 + 8 * 2.0 ** -24)
+    few = pool.rows * (heads // pool.heads) <= 32 * len(pool.keys)
+    grid = 2.0 ** -32 if few else 2.0 ** -23
     weight = 2.0 ** -11 if name != "f32" else 2.0 ** -21
     rel = 2 * score + weight + 2.0 ** -20 + 2 * (keys / 16 + 8) * 2.0 ** -23
-    return rel[..., None] * mag + half_step(name) * np.abs(out) + (2.0 ** -25 if name == "f16" else 1e-30) + keys * 2.0 ** -32 * vmax
+    return rel[..., None] * mag + half_step(name) * np.abs(out) + (2.0 ** -25 if name == "f16" else 1e-30) + keys * grid * vmax / total[..., None]

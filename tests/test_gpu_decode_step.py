@@ -86,8 +86,8 @@ class Layer:
                 codes, sc = int8_rows(c[which][first:first + n].float().numpy())
                 stored = pool.dense(i, which)[pool.keys[i] - n:]
                 assert np.array_equal(stored, codes.astype(np.float64) * sc[..., None].astype(np.float64))
-            want, mag, smag = attention64(pool, c["q"].double().numpy(), HEADS, HD ** -0.5, True, i)
-            tol = attention_tolerance(name, pool, i, want, mag, smag)
+            want, *sizes = attention64(pool, c["q"].double().numpy(), HEADS, HD ** -0.5, True, i)
+            tol = attention_tolerance(name, pool, i, HEADS, want, *sizes)
             assert (np.abs(c["att"][first:first + n].double().numpy() - want) <= tol).all()
         linear("o", c["att"], None, c["o"])
         norm(1, c["o"], c["x"], c["sum1"])

@@ -134,10 +134,10 @@ def compare(pool, out, q, heads, name, scale, causal):
     got, q64 = out.double().cpu().numpy(), q.double().cpu().numpy()
     covered = np.zeros(pool.rows, bool)
     for b in range(len(pool.keys)):
-        want, mag, smag = attention64(pool, q64, heads, scale, causal, b)
+        want, *sizes = attention64(pool, q64, heads, scale, causal, b)
         rows = slice(int(pool.starts[b]), int(pool.starts[b]) + pool.new[b])
         covered[rows] = True
-        tol = attention_tolerance(name, pool, b, want, mag, smag)
+        tol = attention_tolerance(name, pool, b, heads, want, *sizes)
         err = np.abs(got[rows] - want)
         assert (err <= tol).all(), (b, np.nanmax(err / tol), np.isnan(err).sum())
     assert (got[~covered] == 11.0).all()      # rows of no sequence are left alone
@@ -151,6 +151,12 @@ SHAPES = [
     ([5], [5], 4, 1, 16, 128), ([17, 1, 0, 40], [17, 600, 9, 90], 2, 2, 16, 64), ([64], [64], 2, 4, 64, 128),
     ([130], [700], 3, 1, 16, 128), ([65, 63], [1100, 65], 1, 8, 100, 96), ([200, 3], [200, 450], 2, 3, 32, 48),
     ([33], [3000], 24, 1, 64, 128), ([300], [301], 1, 2, 5, 128), ([257, 1], [513, 4000], 2, 4, 128, 128),
+    # enough heads for the tiles of 128 rows, a tile to a block
+    ([70, 5], [333, 640], 24, 4, 16, 128), ([9, 9, 9], [600, 9, 100], 40, 8, 7, 16), ([65], [65], 25, 5, 5, 112),
+    ([2] * 70, list(range(2, 212, 3)), 4, 24, 16, 32), ([1000], [1000], 7, 1, 64, 64), ([33, 0, 40], [900, 5, 41], 30, 2, 100, 48),
+    # few enough tiles for 2, 4 and 8 blocks to share one's keys; blocks that have none
+    ([40, 1, 30], [500, 300, 30], 24, 4, 16, 64), ([130], [2100], 8, 4, 48, 128), ([3, 60], [100, 2500], 16, 2, 64, 80),
+    ([28], [4097], 8, 4, 32, 128), ([257], [1030], 8, 3, 128, 96), ([34, 34], [2049, 34], 7, 3, 33, 16), ([128], [129], 8, 1, 2048, 128),
 ]
 
 
@@ -170,44 +176,44 @@ def test_attention(sdq, name, causal, shape):
 
 
 @pytest.mark.parametrize("name", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("new", [[1, 1], [70, 5]])
-def test_peaked_scores_and_uneven_scales(sdq, name, new):
+@pytest.mark.parametrize("new,kv", [([1, 1], 2), ([70, 5], 2), ([70, 5], 24), ([70, 5], 12)])
+def test_peaked_scores_and_uneven_scales(sdq, name, new, kv):
     """Large logits, and value scales five orders of magnitude apart."""
     rng = np.random.default_rng(31)
-    pool = Pool(sdq, rng, new, [333, 640], 2, 16, 128)
+    pool = Pool(sdq, rng, new, [333, 640], kv, 16, 128)
     pool.fill(rng)
     for s, lo, hi in ((pool.ks, 0, 1.5), (pool.vs, -5, 0)):
         s *= torch.from_numpy(10.0 ** rng.uniform(lo, hi, tuple(s.shape)).astype(np.float32)).cuda()
-    q = torch.from_numpy((2 * rng.standard_normal((pool.rows, 8, 128))).astype(np.float32)).to(DT[name][1]).cuda()
-    out = attend(sdq, pool, q, 8, name, causal=True)
-    compare(pool, out, q, 8, name, 128 ** -0.5, True)
+    q = torch.from_numpy((2 * rng.standard_normal((pool.rows, 4 * kv, 128))).astype(np.float32)).to(DT[name][1]).cuda()
+    out = attend(sdq, pool, q, 4 * kv, name, causal=True)
+    compare(pool, out, q, 4 * kv, name, 128 ** -0.5, True)
 
 
-@pytest.mark.parametrize("new", [[1], [40]])
+@pytest.mark.parametrize("new,kv", [([1], 1), ([40], 1), ([40], 40)])
 @pytest.mark.parametrize("factor", [1e-12, 1e8])
-def test_magnitude_of_q_does_not_matter(sdq, new, factor):
+def test_magnitude_of_q_does_not_matter(sdq, new, kv, factor):
     """q far outside fp16's range, the scale its inverse."""
     rng = np.random.default_rng(32)
-    pool = Pool(sdq, rng, new, [150], 1, 16, 64)
+    pool = Pool(sdq, rng, new, [150], kv, 16, 64)
     pool.fill(rng)
     for name in ("f32", "bf16"):
-        q = torch.from_numpy((factor * rng.standard_normal((pool.rows, 4, 64))).astype(np.float32)).to(DT[name][1]).cuda()
-        out = attend(sdq, pool, q, 4, name, scale=0.125 / factor)
-        compare(pool, out, q, 4, name, 0.125 / factor, False)
+        q = torch.from_numpy((factor * rng.standard_normal((pool.rows, 4 * kv, 64))).astype(np.float32)).to(DT[name][1]).cuda()
+        out = attend(sdq, pool, q, 4 * kv, name, scale=0.125 / factor)
+        compare(pool, out, q, 4 * kv, name, 0.125 / factor, False)
 
 
 def test_extreme_cache_scales(sdq):
     """Scales near fp32's ends: a cache of tiny values, and one whose values are zero."""
     rng = np.random.default_rng(33)
-    for new in ([1, 1], [20, 30]):
+    for new, keys, kv in (([1, 1], [100, 60], 2), ([20, 30], [100, 60], 2), ([20, 30], [100, 60], 52), ([40, 40], [600, 60], 18)):
         for ksc, vsc in ((1e-30, 1e-36), (1e-38, 1e30), (0.0, 0.0), (1.0, 0.0)):
-            pool = Pool(sdq, rng, new, [100, 60], 2, 16, 64)
+            pool = Pool(sdq, rng, new, keys, kv, 16, 64)
             pool.fill(rng)
             pool.ks.fill_(ksc)
             pool.vs.fill_(vsc)
-            q = torch.from_numpy(rng.standard_normal((pool.rows, 4, 64)).astype(np.float32)).cuda()
-            out = attend(sdq, pool, q, 4, "f32", causal=True)
-            compare(pool, out, q, 4, "f32", 0.125, True)
+            q = torch.from_numpy(rng.standard_normal((pool.rows, 2 * kv, 64)).astype(np.float32)).cuda()
+            out = attend(sdq, pool, q, 2 * kv, "f32", causal=True)
+            compare(pool, out, q, 2 * kv, "f32", 0.125, True)
 
 
 @pytest.mark.parametrize("name", ["f32", "bf16"])
@@ -225,18 +231,34 @@ def test_rows_that_see_nothing_are_zero(sdq, name):
     compare(pool, out, q, 4, name, 0.125, False)
 
 
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("last,heads,dim", [(10, 14, 64), (560, 8, 64), (1100, 8, 128)])
+def test_rows_that_see_nothing_in_tiles_of_many_rows(sdq, name, last, heads, dim):
+    """The same with a tile to a block, and with 2 and 4 blocks that share its keys."""
+    rng = np.random.default_rng(36)
+    pool = Pool(sdq, rng, [3, 6, 1, 100], [3, 2, 0, last], heads, 8, dim)
+    pool.fill(rng)
+    q = torch.from_numpy(rng.standard_normal((pool.rows, heads * 4, dim)).astype(np.float32)).to(DT[name][1]).cuda()
+    for causal in (True, False):
+        out = attend(sdq, pool, q, heads * 4, name, causal=causal)
+        assert (out[9] == 0).all() and torch.isfinite(out.float()).all()
+        if causal:
+            assert (out[3:7] == 0).all()
+        compare(pool, out, q, heads * 4, name, dim ** -0.5, causal)
+
+
 def test_nan_in_a_query_stays_in_its_row(sdq):
     rng = np.random.default_rng(35)
-    for new in ([1] * 6, [50]):
-        pool = Pool(sdq, rng, new, [100] * len(new), 2, 16, 128)
+    for new, keys, kv in (([1] * 6, 100, 2), ([50], 100, 2), ([50], 100, 32), ([50], 700, 20)):
+        pool = Pool(sdq, rng, new, [keys] * len(new), kv, 16, 128)
         pool.fill(rng)
         for name in ("f32", "bf16", "f16"):
-            q = torch.from_numpy(rng.standard_normal((pool.rows, 8, 128)).astype(np.float32)).to(DT[name][1]).cuda()
-            clean = attend(sdq, pool, q, 8, name)
+            q = torch.from_numpy(rng.standard_normal((pool.rows, 4 * kv, 128)).astype(np.float32)).to(DT[name][1]).cuda()
+            clean = attend(sdq, pool, q, 4 * kv, name)
             for value in (float("nan"), float("inf")):
                 q2 = q.clone()
                 q2[4, 3, 17] = value
-                out = attend(sdq, pool, q2, 8, name)
+                out = attend(sdq, pool, q2, 4 * kv, name)
                 assert torch.isnan(out[4, 3]).all()
                 out[4, 3] = clean[4, 3]
                 assert torch.equal(out, clean)
@@ -245,15 +267,15 @@ def test_nan_in_a_query_stays_in_its_row(sdq):
 def test_bad_tables_are_not_seen(sdq):
     """Positions without a page take no part; the others are attended to as if they were all."""
     rng = np.random.default_rng(6)
-    for many in (1, 9):
+    for many, heads in ((1, 4), (9, 4), (9, 300)):
         pool = bad_pool(sdq, rng)
         if many > 1:
             pool.new = [n * many for n in pool.new]
             pool.starts = np.concatenate([[0], np.cumsum(pool.new)]).astype(np.int32)
             pool.rows = int(pool.starts[-1])
             pool.refresh()
-        q = torch.from_numpy(rng.standard_normal((pool.rows, 4, 64)).astype(np.float32)).cuda()
-        out = attend(sdq, pool, q, 4, "f32").double().cpu().numpy()
+        q = torch.from_numpy(rng.standard_normal((pool.rows, heads, 64)).astype(np.float32)).cuda()
+        out = attend(sdq, pool, q, heads, "f32").double().cpu().numpy()
         there = {0: [p for p in range(40) if not 8 <= p < 16], 1: list(range(24)), 2: [0, 1], 3: [], 4: list(range(16))}
         for b, pos in there.items():
             rows = slice(int(pool.starts[b]), int(pool.starts[b + 1]))
@@ -263,20 +285,21 @@ def test_bad_tables_are_not_seen(sdq):
             pg, off = pool.table[b, np.array(pos) // 8], np.array(pos) % 8
             k, v = [c.cpu().numpy()[pg, :, off].astype(np.float64) * s.cpu().numpy()[pg, :, off][..., None].astype(np.float64)
                     for c, s in ((pool.k, pool.ks), (pool.v, pool.vs))]
-            for h in range(4):
-                s = 0.125 * (q[rows, h].double().cpu().numpy() @ k[:, h // 2].T)
+            for h in range(heads):
+                s = 0.125 * (q[rows, h].double().cpu().numpy() @ k[:, h * 2 // heads].T)
                 p = np.exp(s - s.max(1, keepdims=True))
-                want = (p / p.sum(1, keepdims=True)) @ v[:, h // 2]
+                want = (p / p.sum(1, keepdims=True)) @ v[:, h * 2 // heads]
                 assert np.max(np.abs(out[rows, h] - want)) <= 1e-5 * np.max(np.abs(v))   # fp32: far above 2^-20
             
 
 @pytest.mark.parametrize("name", ["f32", "bf16"])
-@pytest.mark.parametrize("new", [[1, 1, 1], [30, 50, 1]])
-def test_strided_and_unaligned_queries(sdq, name, new):
+@pytest.mark.parametrize("new,keys,kv", [([1, 1, 1], [60, 77, 9], 2), ([30, 50, 1], [60, 77, 9], 2), ([30, 50, 1], [60, 77, 9], 24),
+                                         ([30, 50, 1], [1060, 77, 9], 11)])
+def test_strided_and_unaligned_queries(sdq, name, new, keys, kv):
     rng = np.random.default_rng(41)
-    pool = Pool(sdq, rng, new, [60, 77, 9], 2, 16, 64)
+    pool = Pool(sdq, rng, new, keys, kv, 16, 64)
     pool.fill(rng)
-    heads = 6
+    heads = 3 * kv
     for ldq, ldo, shift in ((heads * 64 * 2, heads * 64 + 8, 0), (heads * 64 + 3, heads * 64 + 1, 1)):
         flat = torch.from_numpy(rng.standard_normal(pool.rows * ldq + 8).astype(np.float32)).to(DT[name][1]).cuda()
         out = torch.full((pool.rows * ldo + 8,), 11.0, device="cuda").to(DT[name][1])
