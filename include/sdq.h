@@ -356,8 +356,9 @@ SDQ_API int sdq_w4_upload(const uint8_t* q, const void* scale, int scale_dtype, 
  * batch, where the weight's bytes bound a linear.  A is fp32, bf16, fp16, or SDQ_I8 with its row
  * scales (what sdq_rmsnorm_quantize and sdq_quantize_activations make); out is fp32, bf16 or fp16,
  * rounded once; bias is fp32 [N] or NULL.  Products and sums keep fp32's precision for every type of
- * A.  A row of A with a NaN or an infinity gives non-finite outputs in its own row only.  Any M;
- * the weights are read again (from L2 where they fit) for every 8 rows. */
+ * A.  A row of A with a NaN or an infinity gives non-finite outputs in its own row only.  M is at
+ * most 524280 and M * N at most 2^33; the weights are read again (from L2 where they fit) for every 8
+ * rows, so from some tens of rows on an int8 linear (sdq_qgemm) is the faster one. */
 SDQ_API int sdq_w4_matmul(sdq_weight_t w, const void* A_dev, int a_dtype, int64_t lda, const float* a_scale_dev,
                           int64_t M, void* out_dev, int out_dtype, const float* bias_dev, uint32_t flags,
                           void* stream);
@@ -365,7 +366,8 @@ SDQ_API int sdq_w4_matmul(sdq_weight_t w, const void* A_dev, int a_dtype, int64_
 /* A paged int8 key/value cache, in memory that the caller owns.  Each row of head_dim values of one
  * token and head is kept as head_dim int8 and one fp32 scale (max|x| * (1/127), the recipe of
  * sdq_rmsnorm_quantize's rows).  head_dim is a multiple of 16 up to 128;
- * k and v are 16-byte aligned; pages * heads * page_size must fit 31 bits. */
+ * k and v are 16-byte aligned; pages * heads * page_size must fit 31 bits, with heads <= 65535 and
+ * page_size <= 2^24. */
 typedef struct sdq_kv_cache {
   int8_t* k;       /* [pages, heads, page_size, head_dim] */
   int8_t* v;
@@ -380,7 +382,7 @@ typedef struct sdq_kv_cache {
  * decrease; rows in front of row_start[0] and from row_start[batch] on are left alone.  Whatever the
  * tables hold, no kernel leaves the pool: a position whose page number is not in [0, pages), or that
  * lies beyond max_pages pages or below zero, is absent -- append drops it, read gives zeros, and
- * attention does not see it. */
+ * attention does not see it.  batch <= 2^24, and max_pages * page_size must fit 31 bits. */
 typedef struct sdq_kv_seqs {
   const int32_t* row_start;   /* [batch + 1] */
   const int32_t* kv_len;      /* [batch] */
@@ -402,7 +404,9 @@ SDQ_API int sdq_kv_read(const sdq_kv_cache* cache, const sdq_kv_seqs* seqs, void
  * [rows, heads, head_dim] of dtype.  A row sees all kv_len positions of its sequence, with
  * SDQ_CAUSAL only those up to its own; one that sees none gives zeros.  One entry point serves single
  * tokens (row_start = 0, 1, 2, ...) and chunks.  Scores, softmax statistics and sums are fp32; with
- * fp32 q the products keep 22 bits of every factor. */
+ * fp32 q the products keep 22 bits of every factor.  In a chunk, a position's share p * v_scale / sum p
+ * is good to 2^-30 of the sequence's largest v_scale / sum p besides, which shows where the v scales of
+ * one sequence lie many orders apart.  rows * heads <= 2^30, sequences * cache heads <= 2^26, heads <= 65535. */
 SDQ_API int sdq_kv_attention(const sdq_kv_cache* cache, const sdq_kv_seqs* seqs, const void* q_dev, int dtype,
                              int64_t ldq, int64_t rows, int heads, float scale, void* out_dev, int64_t ldo,
                              uint32_t flags, void* stream);

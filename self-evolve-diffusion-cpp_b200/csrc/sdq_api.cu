@@ -856,6 +856,7 @@ int sdq_w4_matmul(sdq_weight_t h, const void* A_dev, int a_dtype, int64_t lda, c
   static const char* const kName = "sdq_w4_matmul";
   return guarded([&]() -> int {
     if (M < 0) return invalid(kName, "negative M");
+    if (M > 65535 * 8) return invalid(kName, "M is too large (this is the few-row product)");   // 65535 blocks of 8 rows
     if (!float_dtype(a_dtype) && a_dtype != SDQ_I8) return invalid(kName, "a_dtype must be SDQ_F32, SDQ_BF16, SDQ_F16 or SDQ_I8");
     if (!float_dtype(out_dtype)) return invalid(kName, "out_dtype must be SDQ_F32, SDQ_BF16 or SDQ_F16");
     if ((a_dtype == SDQ_I8) != (a_scale_dev != nullptr)) return invalid(kName, "a_scale goes with int8 rows, and only with them");
@@ -870,7 +871,7 @@ int sdq_w4_matmul(sdq_weight_t h, const void* A_dev, int a_dtype, int64_t lda, c
     if (M == 0) return SDQ_OK;
     const int64_t ld = lda ? lda : w->K;
     if (ld < w->K) return invalid(kName, "a row stride is shorter than a row");
-    if (M > INT32_MAX || M * w->N > (int64_t(1) << 33)) return invalid(kName, "M is too large (this is the few-row product)");
+    if (M * w->N > (int64_t(1) << 33)) return invalid(kName, "M is too large (this is the few-row product)");
     W4Args a;
     a.q = w->w4; a.scale_dtype = w->w4_scale_dtype; a.group = w->w4_group;
     a.x = A_dev; a.x_dtype = a_dtype; a.ldx = ld; a.x_scale = a_scale_dev; a.bias = bias_dev;

@@ -74,6 +74,7 @@ def test_w4_upload(lib, args, text):
     ((1, P, 0, 0, P, 1, P, 0, None, 0), "a_scale"), ((1, None, 0, 0, None, 1, P, 0, None, 0), "null"),
     ((1, P, 0, 0, None, 1, None, 0, None, 0), "null"), ((1, P, 0, 0, None, 1, P, 0, None, 0x2), "flag"),
     ((1, P + 2, 0, 0, None, 1, P, 0, None, 0), "aligned"), ((1, P, 0, 0, None, 1, P, 0, P + 1, 0), "aligned"),
+    ((1, P, 0, 0, None, 524281, P, 0, None, 0), "too large"),
 ])
 def test_w4_matmul(lib, args, text):
     refused(lib, lib.sdq_w4_matmul(*args, None), text)
