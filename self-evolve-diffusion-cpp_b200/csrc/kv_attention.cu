@@ -486,8 +486,8 @@ __global__ void __launch_bounds__(kBlock, 2) kv_attend_few(const KvArgs a, const
 }
 
 // As many blocks to a sequence and cache head as fill the GPU at two to an SM, and leave a warp a step.
-// One sequence of 32k keys, 8 heads: 247 us with 1 block, 68 with 4, 30.8 with 16; 64 of 4k: 86 with 1,
-// 94 with 2, 118 with 4.
+// One sequence of 32k keys, 8 heads: 246 us with 1 block, 68 with 4, 38 with 8, 31 with 16; 64 of 4k: 75 with
+// 1, 93 with 2, 121 with 4.
 int split_few(const KvArgs& a) {
   int ck = 1;
   const int64_t work = (int64_t)a.batch * a.heads, most = (int64_t)a.max_pages * a.page_size;

@@ -31,7 +31,8 @@
 // the largest error there is (1e-5 of the result at 4k keys).
 //
 // Bound by: the softmax (a block's 128 x 128 weights take 1024 cycles of the exponential unit and ~1200 of
-// issue) with the conversion beside it (~450); the MMAs need 512..1024 per product.
+// issue) with the conversion beside it (~450); the MMAs need 512..1024 per product.  bf16, 3 sequences, 1537
+// rows, 16k keys, 32 query heads on 8: 569 us, 174 at the tensor cores' rate; 496 with the conversion left out.
 //
 // Every mbarrier wait is bounded like the GEMM kernels'.
 #include <cooperative_groups.h>

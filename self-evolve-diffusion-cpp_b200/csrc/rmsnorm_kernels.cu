@@ -244,7 +244,9 @@ cudaError_t launch_typed(const NormArgs& a, cudaStream_t s) {
     const int64_t grid = a.M < 148 * 8 ? a.M : 148 * 8;
     return launch_overlapped(rmsnorm_any<DT>, dim3((unsigned)grid), dim3(kBlock), 0, s, a);
   }
-  // few rows: as many threads to a row as have a vector (latency); many: four vectors to a thread
+  // Few rows: as many threads to a row as have a vector (latency); many: four vectors to a thread.  bf16 rows of
+  // 4096, a vector / four: 1 row 2.1 / 2.9 us, 148 rows 2.3 / 3.4, 296 3.1 / 3.5, 1000 7.8 / 5.7; fp32 rows of
+  // 4096: 2.4 / 2.7, 2.5 / 3.0, 3.7 / 3.3, 10.8 / 6.6.
   if (a.M <= 148 && nv > 64) {
     if (nv <= 256) return launch_regs<DT, 256, 1>(a, s);
     if (nv <= 512) return launch_regs<DT, 512, 1>(a, s);

@@ -516,11 +516,11 @@ bool w4_cut(int64_t N, int64_t K, int rows, int planes, int ring, int ck, int wa
 }
 
 // The cheapest of the four cluster sizes.  A larger cluster means a shorter slice of x to convert in every
-// block and a finer division of the row tiles, and costs a meeting of its blocks.  In clocks, measured:
-// 600 for a tile of a warp (1040 with fp32 rows, two products), 10 / 12 / 56 for 256 elements of x (16
+// block and a finer division of the row tiles, and costs a meeting of its blocks.  In clocks, fitted to
+// such measurements: 600 for a tile of a warp (1040 with fp32 rows, two products), 10 / 12 / 56 for 256 elements of x (16
 // bits / int8 / fp32), 0 / 900 / 1500 / 2000 for the meeting and 8 % for blocks that wait for each other.
-// One row, 4096 x 28672: 14.8 us without clusters, 16.0 / 17.0 / 19.2 with 2 / 4 / 8; 8 fp32 rows,
-// 14336 x 5003: 101 us without, 57 / 36 / 29 with.
+// One bf16 row, 4096 x 28672: 16.5 us without clusters, 16.9 / 17.8 / 19.6 with 2 / 4 / 8; 8 fp32 rows,
+// 14336 x 5003: 51.9 us without, 33.3 / 24.6 / 22.3 with.
 W4Plan w4_plan(const W4Args& a, int rows, int ring, int* smem) {
   const int planes = a.x_dtype == SDQ_F32 ? 2 : 1;
   W4Plan best{};
