@@ -382,7 +382,7 @@ typedef struct sdq_kv_cache {
  * decrease; rows in front of row_start[0] and from row_start[batch] on are left alone.  Whatever the
  * tables hold, no kernel leaves the pool: a position whose page number is not in [0, pages), or that
  * lies beyond max_pages pages or below zero, is absent -- append drops it, read gives zeros, and
- * attention does not see it.  batch <= 2^24, and max_pages * page_size must fit 31 bits. */
+ * attention does not see it.  batch <= 2^24, max_pages * page_size <= 2^30. */
 typedef struct sdq_kv_seqs {
   const int32_t* row_start;   /* [batch + 1] */
   const int32_t* kv_len;      /* [batch] */
@@ -402,7 +402,8 @@ SDQ_API int sdq_kv_read(const sdq_kv_cache* cache, const sdq_kv_seqs* seqs, void
 /* out = softmax(scale * q k^T) v over the cache, for each of `heads` query heads (a multiple of the
  * cache's: query head h reads cache head h / (heads / cache heads)).  q and out are
  * [rows, heads, head_dim] of dtype.  A row sees all kv_len positions of its sequence, with
- * SDQ_CAUSAL only those up to its own; one that sees none gives zeros.  One entry point serves single
+ * SDQ_CAUSAL only those up to its own; one that sees none gives zeros, and what a row does not see
+ * may hold anything, scales that are not finite among it.  One entry point serves single
  * tokens (row_start = 0, 1, 2, ...) and chunks.  Scores, softmax statistics and sums are fp32; with
  * fp32 q the products keep 22 bits of every factor.  In a chunk, a position's share p * v_scale / sum p
  * is good to 2^-30 of the sequence's largest v_scale / sum p besides, which shows where the v scales of

@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kBlock, 2) kv_attend_few(const KvArgs a, const
   const int last_token = (tile.first_row + tile.rows - 1) / group;
   const int last_pos = t.causal ? (int)max((int64_t)-1, (int64_t)table_at(a.kv_len, tile.b) - tile.n + last_token) : INT_MAX;
   const int keys = max(0, t.causal ? (last_pos < tile.len ? last_pos + 1 : tile.len) : tile.len);
-  const int steps = (keys + kStep - 1) / kStep;
+  const int steps = (keys + kStep - 1) / kStep;   // no sequence has more than 2^30 places
   const int per = (steps + ck - 1) / ck;
   const int s0 = min(steps, rank * per), s1 = min(steps, s0 + per);
 
@@ -332,10 +332,19 @@ __global__ void __launch_bounds__(kBlock, 2) kv_attend_few(const KvArgs a, const
         higher |= mn[n][e] > m[n][e];
       }
     }
-    const uint32_t top = __float_as_uint(fmaxf(fmaxf(fabsf(vs[0]), fabsf(vs[1])), fmaxf(fabsf(vs[2]), fabsf(vs[3]))));   // positive floats order as integers
+    auto mag = [&](int i) { return __float_as_uint(vs[i]) & 0x7fffffffu; };   // positive floats order as integers, infinities and NaN last
+    const uint32_t top = max(max(mag(0), mag(1)), max(mag(2), mag(3)));
+    bool odd = false;   // a v scale of the step is not finite (the largest finite one says nothing of it)
     if (__any_sync(0xffffffffu, higher || top > v_top)) {   // rescale what has been summed
       float by = 1.0f;
-      const uint32_t all_top = __reduce_max_sync(0xffffffffu, top);
+      uint32_t all_top = __reduce_max_sync(0xffffffffu, top);
+      odd = all_top >= 0x7f800000u;
+      if (odd) {
+        uint32_t finite = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) finite = max(finite, mag(i) < 0x7f800000u ? mag(i) : 0u);
+        all_top = __reduce_max_sync(0xffffffffu, finite);
+      }
       if (all_top > v_top) {
         v_top = all_top;
         const int e = max((int)(v_top >> 23) - 127 - 14, -126);   // the largest scale into [2^14, 2^15)
@@ -378,6 +387,18 @@ __global__ void __launch_bounds__(kBlock, 2) kv_attend_few(const KvArgs a, const
         if constexpr (P == 2) {
           const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
           pb[i >> 1][P - 1][n][i & 1] = transpose8(half2_bits(wt[0] - back.x, wt[1] - back.y));
+        }
+      }
+    }
+    if (odd && !all) {   // 0 * infinity, which only rows that see the key may have
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          const bool here = (there >> (g + 8 * i)) & 1;
+          const uint32_t keep = transpose8((here && key0 + 8 * i <= pos[n][0] ? 0xffffu : 0u) | (here && key0 + 8 * i <= pos[n][1] ? 0xffff0000u : 0u));
+#pragma unroll
+          for (int p = 0; p < P; p++) pb[i >> 1][p][n][i & 1] &= keep;
         }
       }
     }

@@ -26,13 +26,13 @@
 // weight stays below 2^15 and inside fp16, whose grid ends at 2^-30 of the weight at the offset and of the
 // largest v scale: each key's share is off by 2^-23 of that scale at most, however small its own is.  A larger
 // power than 2^6 would move that down and the offset more often, which scales O and costs as much as a
-// block's exponentials: fp32, 2 x 1000 rows, 8000 keys, 24 heads: 381 us with 2^6, 422 with 2^8, 490 with 2^10.  With fp32 queries O is taken out of tensor memory every kDrain blocks and added up in
+// block's exponentials: fp32, 2 x 1000 rows, 8000 keys, 24 heads: 361 us, 11 % more with 2^8, 29 % with 2^10.  With fp32 queries O is taken out of tensor memory every kDrain blocks and added up in
 // shared memory in fp32: the tensor core's accumulator truncates, and over thousands of keys that would be
 // the largest error there is (1e-5 of the result at 4k keys).
 //
 // Bound by: the softmax (a block's 128 x 128 weights take 1024 cycles of the exponential unit and ~1200 of
 // issue) with the conversion beside it (~450); the MMAs need 512..1024 per product.  bf16, 3 sequences, 1537
-// rows, 16k keys, 32 query heads on 8: 569 us, 174 at the tensor cores' rate; 496 with the conversion left out.
+// rows, 16k keys, 32 query heads on 8: 574 us, 174 at the tensor cores' rate; 496 with the conversion left out.
 //
 // Every mbarrier wait is bounded like the GEMM kernels'.
 #include <cooperative_groups.h>
@@ -62,6 +62,7 @@ constexpr float kStepUp = 9.0f;    // log2 units by which a block's maximum may 
 struct Book {
   float ks[4][kKeys], vs[4][kKeys];   // scales of the blocks under way
   uint32_t there[4][4];               // which of their keys exist
+  uint32_t odd[4][4];                 // which of the v scales are not finite
   int rows[2][4][kKeys];              // pool rows, as the converters of keys and of values looked them up
   float meet[2][2][kRowsT];           // what the two threads of a row tell each other
   float sum[2][kRowsT], off[2][kRowsT];   // sums and offsets of the two halves
@@ -217,6 +218,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
       for (int i = 0; i < 8; i++) {
         const int r = place(p0 + i * kThreadsT);
         x[i] = r >= 0 ? fabsf(__ldg(a.v_scale + r)) : 0.0f;
+        x[i] = x[i] <= 3.402823466e38f ? x[i] : 0.0f;   // an infinity or NaN says nothing of the others
       }
 #pragma unroll
       for (int i = 0; i < 8; i++) top = fmaxf(top, x[i]);
@@ -284,7 +286,11 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
         bk.ks[j & 3][tt] = ks;
         bk.vs[j & 3][tt] = vs * unit;
         const uint32_t there = __ballot_sync(0xffffffffu, row_now >= 0);
-        if (lane == 0) bk.there[j & 3][warp - 8] = there;
+        const uint32_t odd = __ballot_sync(0xffffffffu, !(fabsf(vs) <= 3.402823466e38f));
+        if (lane == 0) {
+          bk.there[j & 3][warp - 8] = there;
+          bk.odd[j & 3][warp - 8] = odd;
+        }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -666,6 +672,26 @@ __global__ void __launch_bounds__(kThreadsT, 1) kv_attend_many(const KvArgs a, c
         }
       }
       l += (lb[0] + lb[1]) + (lb[2] + lb[3]);
+      if (!all && (bk.odd[j & 3][grp * 2] | bk.odd[j & 3][grp * 2 + 1]) != 0) {
+        // 0 * infinity, which only rows that see the key may have.  Rare, so the weights are taken back for it:
+        // a choice at each of them above took 3 to 7 % of all calls.
+        tmem_st_wait();
+#pragma unroll 1
+        for (int h = 0; h < 2; h++) {
+          const int left_h = seen - (j * kKeys + grp * 64) - 32 * h;
+          const uint32_t sees_h = bk.there[j & 3][grp * 2 + h] & (left_h >= 32 ? 0xffffffffu : left_h <= 0 ? 0u : (1u << left_h) - 1);
+          uint32_t w[32];
+          tmem_ld_32x32(s_col + 32 * h, w);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const uint32_t keep = ((sees_h >> (2 * i)) & 1 ? 0xffffu : 0u) | ((sees_h >> (2 * i + 1)) & 1 ? 0xffff0000u : 0u);
+            w[i] &= keep;
+            if constexpr (P == 2) w[16 + i] &= keep;
+          }
+          tmem_st_32x32(s_col + 32 * h, w);
+        }
+      }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();

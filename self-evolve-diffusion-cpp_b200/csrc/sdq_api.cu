@@ -888,7 +888,7 @@ static const char* kv_args(const sdq_kv_cache* c, const sdq_kv_seqs* s, int64_t 
   if (c->head_dim < 16 || c->head_dim > 128 || c->head_dim % 16 != 0) return "head_dim must be a multiple of 16 up to 128";
   if (c->heads > 65535 || c->page_size > (1 << 24) || c->pages > INT32_MAX / ((int64_t)c->heads * c->page_size))
     return "pages * heads * page_size must fit 31 bits";
-  if (s->batch < 0 || s->batch > (1 << 24) || s->max_pages < 0 || (int64_t)s->max_pages * c->page_size > INT32_MAX) return "bad sequence table shape";
+  if (s->batch < 0 || s->batch > (1 << 24) || s->max_pages < 0 || (int64_t)s->max_pages * c->page_size > (1 << 30)) return "bad sequence table shape";
   if (rows < 0 || rows > INT32_MAX / 2) return "bad number of rows";
   if (c->pages > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale)) return "null pointer in the cache";
   if (s->batch > 0 && (!s->row_start || !s->kv_len || (s->max_pages > 0 && !s->page_table))) return "null pointer in the sequence table";

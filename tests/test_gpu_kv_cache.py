@@ -264,6 +264,32 @@ def test_nan_in_a_query_stays_in_its_row(sdq):
                 assert torch.equal(out, clean)
 
 
+@pytest.mark.parametrize("name", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("new,keys,kv,group", [([5], [100], 2, 2), ([40], [130], 1, 1), ([60], [400], 50, 4), ([60], [1000], 20, 4)])
+def test_scales_that_are_not_finite_stay_with_the_rows_that_see_them(sdq, name, new, keys, kv, group):
+    """A key that a causal row does not see may hold anything; the rows that see it have no finite answer."""
+    rng = np.random.default_rng(37)
+    pool = Pool(sdq, rng, new, keys, kv, 16, 64)
+    pool.fill(rng)
+    heads = kv * group
+    q = torch.from_numpy(rng.standard_normal((pool.rows, heads, 64)).astype(np.float32)).to(DT[name][1]).cuda()
+    want, *sizes = attention64(pool, q.double().cpu().numpy(), heads, 0.125, True, 0)
+    before = new[0] - 3                  # the third-last position is not seen by the rows before it
+    tol = attention_tolerance(name, pool, 0, heads, want, *sizes)[:before]
+    pg, off = pool.places(0)
+    place = int(pg[keys[0] - 3]), slice(None), int(off[keys[0] - 3])
+    first = int(pool.starts[0])
+    for which in (pool.ks, pool.vs):
+        keep = which[place].clone()
+        for value in (float("nan"), float("inf")):
+            which[place] = value
+            out = attend(sdq, pool, q, heads, name, causal=True)
+            assert (np.abs(out[first:first + before].double().cpu().numpy() - want[:before]) <= tol).all()
+            if which is pool.vs:
+                assert not torch.isfinite(out[first + before:first + new[0]]).any()
+        which[place] = keep
+
+
 def test_bad_tables_are_not_seen(sdq):
     """Positions without a page take no part; the others are attended to as if they were all."""
     rng = np.random.default_rng(6)
