@@ -516,22 +516,31 @@ int split_few(const KvArgs& a) {
   return ck;
 }
 
+template <int NJ, int NT>
+constexpr int kSmemFew = kWarps * kDepth * Stage<NJ>::kBytes > kWarps * 8 * NT * 64 * NJ * 4 ? kWarps * kDepth * Stage<NJ>::kBytes
+                                                                                            : kWarps * 8 * NT * 64 * NJ * 4;
+template <int DT, int NJ, int NT>
+cudaError_t allow_few() {
+  const cudaError_t e = cudaFuncSetAttribute(kv_attend_few<DT, NJ, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemFew<NJ, NT>);
+  return e != cudaSuccess ? e : cudaFuncSetAttribute(kv_attend_few<DT, NJ, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
+template <int DT>
+cudaError_t allow_typed() {
+  cudaError_t e = allow_few<DT, 1, 1>();
+  if (e == cudaSuccess) e = allow_few<DT, 1, 2>();
+  if (e == cudaSuccess) e = allow_few<DT, 2, 1>();
+  return e == cudaSuccess ? allow_few<DT, 2, 2>() : e;
+}
+
 template <int DT, int NJ, int NT>
 cudaError_t launch_few(const KvArgs& a, const AttendArgs& t, int vec, cudaStream_t s) {
   const int group = t.heads / a.heads;
   const int64_t tiles = (int64_t)a.rows * group / (8 * NT) + a.batch;   // with numbers that are no tile, see Tile
   const int ck = split_few(a);
-  constexpr int kSmem = kWarps * kDepth * Stage<NJ>::kBytes > kWarps * 8 * NT * 64 * NJ * 4 ? kWarps * kDepth * Stage<NJ>::kBytes
-                                                                                         : kWarps * 8 * NT * 64 * NJ * 4;
-  static const cudaError_t set = [] {
-    const cudaError_t e = cudaFuncSetAttribute(kv_attend_few<DT, NJ, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    return e != cudaSuccess ? e : cudaFuncSetAttribute(kv_attend_few<DT, NJ, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  }();
-  if (set != cudaSuccess) return set;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * a.heads * ck));
   cfg.blockDim = dim3(kBlock);
-  cfg.dynamicSmemBytes = kSmem;
+  cfg.dynamicSmemBytes = kSmemFew<NJ, NT>;
   cfg.stream = s;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -554,6 +563,17 @@ cudaError_t launch_typed(const KvArgs& a, const AttendArgs& t, cudaStream_t s) {
 }
 
 }  // namespace
+
+int kv_attend_few_setup(std::string* why) {
+  cudaError_t e = allow_typed<SDQ_F32>();
+  if (e == cudaSuccess) e = allow_typed<SDQ_BF16>();
+  if (e == cudaSuccess) e = allow_typed<SDQ_F16>();
+  if (e != cudaSuccess) {
+    if (why) *why = std::string("cache attention set-up: ") + cudaGetErrorString(e);
+    return SDQ_ERR_CUDA;
+  }
+  return SDQ_OK;
+}
 
 cudaError_t launch_kv_attention(const KvArgs& a, const AttendArgs& t, int dtype, cudaStream_t s) {
   count_launch();

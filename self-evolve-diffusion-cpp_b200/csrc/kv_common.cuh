@@ -191,6 +191,8 @@ cudaError_t launch_kv_io(const KvArgs& a, void* k, void* v, int dtype, int64_t l
 cudaError_t launch_kv_attention(const KvArgs& a, const AttendArgs& t, int dtype, cudaStream_t s);
 // the many-row kernel on tcgen05: kv_attention_tcgen05.cu
 cudaError_t launch_kv_attend_many(const KvArgs& a, const AttendArgs& t, int dtype, cudaStream_t s);
+// at sdq_init, for its device: the kernels' shared memory and cluster sizes
+int kv_attend_few_setup(std::string* why);
 int kv_attend_many_setup(std::string* why);
 
 }  // namespace sdq

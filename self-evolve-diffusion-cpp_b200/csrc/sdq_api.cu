@@ -314,7 +314,9 @@ int sdq_init(int device) {
   int rc = qgemm_tc_setup(&why);
   if (rc == SDQ_OK) rc = fgemm_setup(&why);
   if (rc == SDQ_OK) rc = sdpa_setup(&why);
+  if (rc == SDQ_OK) rc = kv_attend_few_setup(&why);
   if (rc == SDQ_OK) rc = kv_attend_many_setup(&why);
+  if (rc == SDQ_OK) rc = w4_setup(&why);
   if (rc != SDQ_OK) { cudaFree(c->status); delete c; return fail(rc, why); }
   g_ctx = c;
   return SDQ_OK;

@@ -153,6 +153,7 @@ cudaError_t launch_w4_quantize(const void* src, int src_dtype, int64_t N, int64_
 // packed rows (low nibble first) + scales [N, groups], device memory, into the tile layout
 cudaError_t launch_w4_layout(const uint8_t* q, const void* scale, int scale_dtype, int64_t N, int64_t K, int group,
                              uint32_t* out, cudaStream_t s);
+int w4_setup(std::string* why);   // at sdq_init, for its device
 cudaError_t launch_w4_matmul(const W4Args& a, cudaStream_t s);
 
 // MMA-issue-bound int8 rate of the device (mma_probe.cu).

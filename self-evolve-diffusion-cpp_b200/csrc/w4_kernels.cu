@@ -542,8 +542,6 @@ template <int XT, int ST, int GROUP>
 cudaError_t launch_rows(const W4Args& a, cudaStream_t s) {
   int smem = 0;
   const W4Plan p = w4_plan(a, (int)std::min<int64_t>(a.M, kRows), kAhead * kTileBytes(ST == SDQ_F32 ? 4 : 2, GROUP), &smem);
-  static const cudaError_t set = cudaFuncSetAttribute(w4_rows_kernel<XT, ST, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
-  if (set != cudaSuccess) return set;
   const int n_tiles = (int)((a.N + 15) / 16);
   const int strips = p.strips_long + (n_tiles - p.strips_long * p.strip) / std::max(1, p.strip - 1);
   const int size = XT == SDQ_F32 ? 4 : XT == SDQ_I8 ? 1 : 2;
@@ -561,6 +559,22 @@ cudaError_t launch_rows(const W4Args& a, cudaStream_t s) {
   cfg.attrs = at;
   cfg.numAttrs = p.ck > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, w4_rows_kernel<XT, ST, GROUP>, a, p, vec);
+}
+template <int XT, int ST, int GROUP>
+cudaError_t allow_rows() {
+  return cudaFuncSetAttribute(w4_rows_kernel<XT, ST, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+}
+template <int XT, int ST>
+cudaError_t allow_group() {
+  cudaError_t e = allow_rows<XT, ST, 32>();
+  if (e == cudaSuccess) e = allow_rows<XT, ST, 64>();
+  return e == cudaSuccess ? allow_rows<XT, ST, 128>() : e;
+}
+template <int XT>
+cudaError_t allow_scales() {
+  cudaError_t e = allow_group<XT, SDQ_F32>();
+  if (e == cudaSuccess) e = allow_group<XT, SDQ_BF16>();
+  return e == cudaSuccess ? allow_group<XT, SDQ_F16>() : e;
 }
 template <int XT, int ST>
 cudaError_t launch_group(const W4Args& a, cudaStream_t s) {
@@ -605,6 +619,18 @@ cudaError_t launch_w4_layout(const uint8_t* q, const void* scale, int scale_dtyp
   if (scale_dtype == SDQ_F32) w4_layout_kernel<4><<<grid, kBlock, 0, s>>>(q, scale, N, K, group, tile_words, words, out);
   else w4_layout_kernel<2><<<grid, kBlock, 0, s>>>(q, scale, N, K, group, tile_words, words, out);
   return cudaGetLastError();
+}
+
+int w4_setup(std::string* why) {
+  cudaError_t e = allow_scales<SDQ_F32>();
+  if (e == cudaSuccess) e = allow_scales<SDQ_BF16>();
+  if (e == cudaSuccess) e = allow_scales<SDQ_F16>();
+  if (e == cudaSuccess) e = allow_scales<SDQ_I8>();
+  if (e != cudaSuccess) {
+    if (why) *why = std::string("4-bit product set-up: ") + cudaGetErrorString(e);
+    return SDQ_ERR_CUDA;
+  }
+  return SDQ_OK;
 }
 
 cudaError_t launch_w4_matmul(const W4Args& a, cudaStream_t s) {
